@@ -512,6 +512,132 @@ int mt_causal_conv1d(const void* x, const void* weight, const void* bias,
                      void* conv_state, void* y, int64_t L, int64_t C,
                      int width, int silu, int dtype, mt_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Paged serving: one step of a batch of requests over a paged KV cache       */
+/* ------------------------------------------------------------------------ */
+/*
+ * The reference serves one request at a time from a dense cache
+ * (autotuner_runtime/inference.py:131-156); these entry points have no
+ * counterpart there. They run one step of a batch: mt_paged_plan once per
+ * step, mt_rope_paged_append and mt_paged_sdpa_decode once per layer,
+ * mt_token_logprobs on the step's logits. All lengths, tables and slots stay
+ * on the device, so a step can be captured in a CUDA graph and replayed.
+ *
+ * A cache is `num_pages` pages of `page_size` rows for each of Hkv heads:
+ * element (page, head, slot, d) at page*page_stride + head*head_stride +
+ * slot*slot_stride + d (strides in elements, multiples of 8; both [pages,
+ * heads, slots, D] and [pages, slots, heads, D] are such layouts). A slot
+ * number is page * page_size + row.
+ */
+
+/*
+ * The step's plan from request lengths. Request r has ctx_lens[r] tokens in
+ * the cache and brings new_lens[r] more (negative lengths count as 0); its
+ * new tokens follow those of request r-1 in the step's flat token order.
+ *   block_table [B, max_pages] (row stride table_stride): holds the pages of
+ *               the cached tokens; entries for the pages the new tokens need
+ *               are written, taken in request order from
+ *               free_pages[*free_head ..] (free_head NULL: from the start).
+ *               It is updated in place, nothing else of it is touched.
+ *   seq_lens    [B]    ctx + new (ctx alone for a refused request)
+ *   query_start [B+1]  first token of each request; the total at the end
+ *   positions, token_seq, slots [token_cap]  each token's position in its
+ *               request, request, and slot (-1: no slot); past the last
+ *               token 0, -1, -1
+ *   counts      [5]    tokens, pages wanted, pages taken, requests refused,
+ *               and the free-list head after the step
+ * A request is refused (no page, slots -1) when its tokens end past
+ * token_cap, when ctx + new exceeds max_pages * page_size (or 2^31 - 1), or
+ * when its pages end past the n_free pages of the list; the requests after
+ * one that ran out of pages get none either, so pages are dealt in order.
+ * The same inputs give the same plan again: no input but the table is
+ * written, and only entries past the cached tokens. Output lengths, the head
+ * and the counts are the inputs of the next step. Sums saturate at 2^31 - 1.
+ */
+int mt_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int64_t B,
+                  int32_t* block_table, int64_t table_stride, int64_t max_pages,
+                  const int32_t* free_pages, int64_t n_free,
+                  const int32_t* free_head, int64_t page_size,
+                  int64_t token_cap, int32_t* seq_lens, int32_t* query_start,
+                  int32_t* positions, int32_t* token_seq, int64_t* slots,
+                  int32_t* counts, mt_stream_t stream);
+
+/*
+ * q/k prologue of a batch and the append to the paged cache, one launch.
+ * For token t (position positions[t], slot slots[t]) and each head row of D
+ * values: optional RMSNorm (q_norm_w / k_norm_w [D], NULL: none), then rotary
+ * position embedding of the first `dims` values,
+ *   a_j = position * inv_freq[j], j < dims/2
+ *   (y_i, y_j') = mscale * (x_i cos a_j - x_j' sin a_j, x_j' cos a_j + x_i sin a_j)
+ * with pairs (j, j + dims/2), or (2j, 2j + 1) when `traditional`; the values
+ * past `dims` are copied. inv_freq (fp32, device) carries any base and any
+ * scaling rule for long contexts; mscale its magnitude factor (1: none).
+ * Arithmetic in fp32 (the angle reduced in fp64), rounded once: unlike
+ * mt_qk_norm_rope_cache, which rounds after the norm as the separate MLX ops do.
+ *   q [T, Hq, D], k, v [T, Hkv, D]  strides (token, head) in elements, D
+ *          contiguous; rows 16-byte aligned, strides multiples of 8
+ *   q_out  [T, Hq, D] with strides qo_st, qo_sh; may be q with q's strides
+ *   k_out  [T, Hkv, D] dense rotated k rows, or NULL
+ *   caches as above; a row with slot < 0 is not written there, one past the
+ *          last page is not written and is reported through the device status
+ * D a multiple of 8 up to 256, dims even; bf16, f16 or f32. Two rows with one
+ * slot leave either.
+ */
+int mt_rope_paged_append(
+    const void* q, const void* k, const void* v, int64_t q_st, int64_t q_sh,
+    int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+    const void* q_norm_w, const void* k_norm_w, float eps,
+    const int32_t* positions, const int64_t* slots, const float* inv_freq,
+    int dims, int traditional, float mscale, void* q_out, int64_t qo_st,
+    int64_t qo_sh, void* k_out, void* k_cache, void* v_cache,
+    int64_t num_pages, int64_t page_size, int64_t page_stride,
+    int64_t head_stride, int64_t slot_stride, int64_t T, int64_t Hq,
+    int64_t Hkv, int64_t D, int dtype, mt_stream_t stream);
+
+/*
+ * Attention of one new token per request over its pages:
+ *   o[b,h] = sum_i softmax_i(scale q[b,h] . k_i) v_i,  i < seq_lens[b]
+ * with key row i at page block_table[b, i / page_size], row i % page_size, kv
+ * head h / (Hq / Hkv). q and o [B, Hq, D] with strides (request, head), D
+ * contiguous (q rows 4-byte, o rows 8-byte aligned); D = 64 or 128; bf16 or
+ * f16; any page_size. A length of 0 (or less) gives zeros; lengths past
+ * max_pages * page_size are cut there. A page id outside the cache hides its
+ * keys and is reported through the device status. Scores, softmax sums and
+ * outputs are accumulated in fp32, the probabilities rounded to dtype for the
+ * product with v. The work is split over the keys, so a request's sums may
+ * be grouped differently beside other requests; the same call repeats bitwise.
+ * The workspace holds parts of split requests and arrival counters: a zeroed
+ * one as described above; concurrent calls need workspaces of their own.
+ */
+size_t mt_paged_sdpa_decode_workspace_bytes(int64_t D);
+
+int mt_paged_sdpa_decode(
+    const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache,
+    const void* v_cache, int64_t num_pages, int64_t page_size,
+    int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+    const int32_t* block_table, int64_t table_stride, int64_t max_pages,
+    const int32_t* seq_lens, void* o, int64_t o_sb, int64_t o_sh, int64_t B,
+    int64_t Hq, int64_t Hkv, int64_t D, float scale, int dtype, void* workspace,
+    size_t workspace_bytes, mt_stream_t stream);
+
+/*
+ * Per row of logits [R, V] (row_stride elements apart): lse = logsumexp,
+ * logprob = logits[tokens[r]] - lse (tokens NULL: not computed; an id < 0 is
+ * padding and gives 0, an id >= V gives 0 and is reported through the device
+ * status), entropy = -sum p log p, and the top_k values in falling order
+ * (ties: lower id first; NaN before every number) with ids top_ids and
+ * log-probabilities top_logprobs [R, top_k]. entropy and lse may be NULL.
+ * bf16, f16 or f32 in, fp32 out; nothing is rounded to the logits' type
+ * (mt_logits_pick does, as mlx-lm). -inf logits have probability 0; a row
+ * that holds NaN or +inf, or only -inf, has no distribution and gives NaN.
+ * 0 <= top_k <= 32.
+ */
+int mt_token_logprobs(const void* logits, int64_t row_stride,
+                      const int32_t* tokens, int64_t R, int64_t V, int top_k,
+                      float* logprob, float* entropy, float* lse,
+                      int32_t* top_ids, float* top_logprobs, int dtype,
+                      mt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

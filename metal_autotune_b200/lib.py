@@ -9,8 +9,10 @@ device, the call raises.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import threading
 from pathlib import Path
+from typing import NamedTuple
 
 import torch
 
@@ -98,6 +100,15 @@ SIGNATURES = {
     "mt_layer_norm": (C.c_int, [P, P, P, F32, P, I64, I64, I32, P]),
     "mt_mamba_scan": (C.c_int, [P, P, P, P, P, P, P, P, P, P, I64, I64, I64, I32, P]),
     "mt_causal_conv1d": (C.c_int, [P, P, P, P, P, I64, I64, I32, I32, I32, P]),
+    "mt_paged_plan": (C.c_int, [P, P, I64, P, I64, I64, P, I64, P, I64, I64, P, P, P, P, P, P, P]),
+    "mt_rope_paged_append": (
+        C.c_int, [P, P, P, I64, I64, I64, I64, I64, I64, P, P, F32, P, P, P, I32, I32, F32, P, I64, I64, P, P, P,
+                  I64, I64, I64, I64, I64, I64, I64, I64, I64, I32, P]),
+    "mt_paged_sdpa_decode_workspace_bytes": (C.c_size_t, [I64]),
+    "mt_paged_sdpa_decode": (
+        C.c_int, [P, I64, I64, P, P, I64, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, I64, I64, I64, I64, F32,
+                  I32, P, SZ, P]),
+    "mt_token_logprobs": (C.c_int, [P, I64, P, I64, I64, I32, P, P, P, P, P, I32, P]),
 }
 
 _lib = None
@@ -535,6 +546,232 @@ def causal_conv1d(x, weight, bias=None, *, conv_state=None, silu=True, out=None)
     call("mt_causal_conv1d", _ptr(x), _ptr(weight), _ptr(bias), _ptr(conv_state), _ptr(y), L, Cn, width,
          int(bool(silu)), dtype_code(x.dtype), _stream())
     return y
+
+
+# ------------------------------------------------------------------ paged serving
+class PagedPlan(NamedTuple):
+    """One step's plan (mt_paged_plan): see `paged_plan`."""
+    seq_lens: torch.Tensor
+    query_start: torch.Tensor
+    positions: torch.Tensor
+    token_seq: torch.Tensor
+    slots: torch.Tensor
+    counts: torch.Tensor
+
+    @classmethod
+    def empty(cls, requests: int, token_cap: int, device="cuda") -> "PagedPlan":
+        i32 = lambda n: torch.empty(n, dtype=torch.int32, device=device)  # noqa: E731
+        return cls(i32(requests), i32(requests + 1), i32(token_cap), i32(token_cap),
+                   torch.empty(token_cap, dtype=torch.int64, device=device), i32(5))
+
+
+def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple | None = None) -> torch.Tensor:
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return _dense(t, name)
+
+
+def paged_plan(ctx_lens, new_lens, block_table, free_pages, *, page_size, token_cap, free_head=None, out=None):
+    """Plan one step of a batch: where its new tokens go in the paged cache.
+
+    ctx_lens / new_lens int32 [B]; block_table int32 [B, max_pages] (rows may be strided), updated in
+    place with the new pages; free_pages int32 [n], taken from *free_head (int32 [1], default 0) on.
+    Returns a PagedPlan (`out`, from PagedPlan.empty(B, token_cap), or a new one): seq_lens [B],
+    query_start [B+1], positions / token_seq int32 and slots int64 [token_cap] (slot -1: padding or a
+    refused request), counts [5] = tokens, pages wanted, pages taken, requests refused, next free_head."""
+    B = ctx_lens.shape[0]
+    i32 = torch.int32
+    _want(ctx_lens, "ctx_lens", i32, (B,))
+    _want(new_lens, "new_lens", i32, (B,))
+    _want(free_pages, "free_pages", i32)
+    if free_head is not None:
+        _want(free_head, "free_head", i32, (1,))
+    if block_table.dtype is not i32 or block_table.dim() != 2 or block_table.shape[0] != B or (
+            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be int32 [{B}, max_pages] with contiguous rows")
+    if out is None:
+        out = PagedPlan.empty(B, token_cap, ctx_lens.device)
+    else:
+        for t, name, dt, n in zip(out, PagedPlan._fields, (i32, i32, i32, i32, torch.int64, i32),
+                                  (B, B + 1, token_cap, token_cap, token_cap, 5)):
+            _want(t, f"out.{name}", dt, (n,))
+    width = block_table.shape[1]
+    call("mt_paged_plan", _ptr(ctx_lens), _ptr(new_lens), B, _ptr(block_table),
+         block_table.stride(0) if B > 1 else max(width, block_table.stride(0)), width, _ptr(free_pages),
+         free_pages.numel(), _ptr(free_head), int(page_size), int(token_cap), _ptr(out.seq_lens),
+         _ptr(out.query_start), _ptr(out.positions), _ptr(out.token_seq), _ptr(out.slots), _ptr(out.counts),
+         _stream())
+    return out
+
+
+def rope_frequencies(dims, *, base=10000.0, scaling=None, device="cuda"):
+    """(inv_freq fp32 [dims/2] on `device`, mscale) for `rope_paged_append`.
+
+    scaling None: base^(-2j/dims). Otherwise a dict with "type" and "factor":
+      "linear"  every angle divided by factor
+      "llama3"  wavelengths beyond original_max_position / low_freq_factor divided by factor, those within
+                original_max_position / high_freq_factor kept, between them interpolated
+      "yarn"    dimensions that turn fewer than beta_slow times over original_max_position divided by
+                factor, those that turn more than beta_fast times kept, a linear ramp over the dimension
+                between; mscale = 0.1 ln(factor) + 1
+    """
+    half = dims // 2
+    if dims < 0 or dims % 2:
+        raise ValueError(f"dims={dims} must be even")
+    freqs = [float(base) ** (-2.0 * j / dims) for j in range(half)]
+    mscale = 1.0
+    if scaling is not None:
+        kind, factor = scaling["type"], float(scaling["factor"])
+        if factor <= 0:
+            raise ValueError(f"factor={factor} must be positive")
+        if kind == "linear":
+            freqs = [f / factor for f in freqs]
+        elif kind == "llama3":
+            old = float(scaling.get("original_max_position", 8192))
+            low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+            if high <= low:
+                raise ValueError(f"high_freq_factor={high} must exceed low_freq_factor={low}")
+            keep = [min(1.0, max(0.0, (old * f / (2 * math.pi) - low) / (high - low))) for f in freqs]
+            freqs = [f * k + f / factor * (1.0 - k) for f, k in zip(freqs, keep)]
+        elif kind == "yarn":
+            old = float(scaling.get("original_max_position", 8192))
+            fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+            at = lambda turns: dims * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+            lo, hi = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), dims - 1)
+            ramp = [min(1.0, max(0.0, (j - lo) / max(hi - lo, 1e-3))) for j in range(half)]
+            freqs = [f * (1.0 - r) + f / factor * r for f, r in zip(freqs, ramp)]
+            mscale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+        else:
+            raise ValueError(f"unknown rope scaling {kind!r}")
+    return torch.tensor(freqs, dtype=torch.float32, device=device), mscale
+
+
+def _check_cache(k_cache, v_cache, dtype):
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        raise ValueError("k_cache and v_cache must be [pages, Hkv, page_size, D] of one shape and strides")
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
+        raise TypeError(f"the caches must be {dtype}, as q")
+    if k_cache.stride(3) != 1:
+        raise ValueError("the caches' rows (D) must be contiguous")
+
+
+def rope_paged_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq, *, traditional=False, mscale=1.0,
+                      q_norm_w=None, k_norm_w=None, eps=1e-6, out=None, k_out=None):
+    """Optional q/k RMSNorm, rotary embedding of the first 2*len(inv_freq) values of each head at
+    positions[t], and the append of k and v to slots[t] of the paged cache, in one launch.
+
+    q [T, Hq, D], k / v [T, Hkv, D] (D contiguous, any token and head strides, e.g. views of one
+    projection's rows); positions int32 [T], slots int64 [T] (negative: not written); caches
+    [pages, Hkv, page_size, D] (or a permuted view of that shape). Returns the rotated q, dense
+    [T, Hq, D] or `out` (which may be q). `k_out` dense [T, Hkv, D] also receives the rotated k."""
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    dt = q.dtype
+    if k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D) or k.dtype is not dt or v.dtype is not dt:
+        raise ValueError(f"k and v must be {dt} [{T}, Hkv, {D}]")
+    if q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("q, k and v must have D contiguous")
+    _check_cache(k_cache, v_cache, dt)
+    if k_cache.shape[1] != Hkv or k_cache.shape[3] != D:
+        raise ValueError(f"the caches must be [pages, {Hkv}, page_size, {D}]")
+    _want(positions, "positions", torch.int32, (T,))
+    _want(slots, "slots", torch.int64, (T,))
+    _want(inv_freq, "inv_freq", torch.float32)
+    for w, name in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
+        if w is not None:
+            _want(w, name, dt, (D,))
+    y = out if out is not None else torch.empty((T, Hq, D), dtype=dt, device=q.device)
+    if y is not q and (y.shape != q.shape or y.dtype is not dt or y.stride(2) != 1):
+        raise ValueError("out must have q's shape and dtype with D contiguous")
+    if k_out is not None:
+        _want(k_out, "k_out", dt, (T, Hkv, D))
+    call("mt_rope_paged_append", _ptr(q), _ptr(k), _ptr(v), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+         v.stride(0), v.stride(1), _ptr(q_norm_w), _ptr(k_norm_w), float(eps), _ptr(positions), _ptr(slots),
+         _ptr(inv_freq), 2 * inv_freq.shape[0], int(bool(traditional)), float(mscale), _ptr(y), y.stride(0),
+         y.stride(1), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], k_cache.shape[2],
+         k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), T, Hq, Hkv, D, dtype_code(dt), _stream())
+    return y
+
+
+def paged_sdpa_decode(q, k_cache, v_cache, block_table, seq_lens, *, scale, out=None, workspace=None):
+    """Attention of one new token per request over its pages: q [B, Hq, D], caches [pages, Hkv,
+    page_size, D] (or a permuted view of that shape), block_table int32 [B, max_pages], seq_lens int32
+    [B] (0: that request's output is zeros). Returns [B, Hq, D]. `workspace`: a Workspace of the
+    caller's own, for calls on a stream other than the one that uses the device's shared workspace."""
+    B, Hq, D = q.shape
+    dt = q.dtype
+    _check_cache(k_cache, v_cache, dt)
+    pages, Hkv, page_size, _ = k_cache.shape
+    if k_cache.shape[3] != D:
+        raise ValueError(f"the caches must be [pages, Hkv, page_size, {D}]")
+    if q.stride(2) != 1:
+        raise ValueError("q must have D contiguous")
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or (
+            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be int32 [{B}, max_pages] with contiguous rows")
+    _want(seq_lens, "seq_lens", torch.int32, (B,))
+    o = out if out is not None else torch.empty((B, Hq, D), dtype=dt, device=q.device)
+    if o.shape != q.shape or o.dtype is not dt or o.stride(2) != 1:
+        raise ValueError("out must have q's shape and dtype with D contiguous")
+    ws = workspace if workspace is not None else Workspace.get(_paged_ws_bytes(D))
+    width = block_table.shape[1]
+    call("mt_paged_sdpa_decode", _ptr(q), q.stride(0), q.stride(1), _ptr(k_cache), _ptr(v_cache), pages, page_size,
+         k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), _ptr(block_table),
+         block_table.stride(0) if B > 1 else max(width, block_table.stride(0)), width, _ptr(seq_lens), _ptr(o),
+         o.stride(0), o.stride(1), B, Hq, Hkv, D, float(scale), dtype_code(dt), ws.ptr, ws.nbytes, _stream())
+    return o
+
+
+_paged_ws: dict[int, int] = {}
+
+
+def _paged_ws_bytes(D: int) -> int:
+    n = _paged_ws.get(D)
+    if n is None:
+        n = _paged_ws[D] = int(load().mt_paged_sdpa_decode_workspace_bytes(D))
+    return n
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row of logits: see `token_logprobs`."""
+    logprob: torch.Tensor | None
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+    @classmethod
+    def empty(cls, rows: int, top_k: int, device="cuda", tokens: bool = True) -> "TokenLogprobs":
+        f32 = lambda *s: torch.empty(*s, dtype=torch.float32, device=device)  # noqa: E731
+        return cls(f32(rows) if tokens else None, f32(rows), f32(rows),
+                   torch.empty(rows, top_k, dtype=torch.int32, device=device), f32(rows, top_k))
+
+
+def token_logprobs(logits, tokens=None, *, top_k=0, out=None):
+    """Log-probability of tokens[r] under row r of logits [R, V] (rows may be strided), with the row's
+    entropy, logsumexp and top_k alternatives (ids and log-probabilities in falling order, ties to the
+    lower id). tokens int32 [R] (negative: 0) or None; fp32 results in a TokenLogprobs (`out`, from
+    TokenLogprobs.empty(R, top_k), or a new one)."""
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be [R, V] with contiguous rows")
+    R, V = logits.shape
+    if tokens is not None:
+        _want(tokens, "tokens", torch.int32, (R,))
+    if out is None:
+        out = TokenLogprobs.empty(R, top_k, logits.device, tokens is not None)
+    else:
+        if tokens is not None:
+            _want(out.logprob, "out.logprob", torch.float32, (R,))
+        _want(out.entropy, "out.entropy", torch.float32, (R,))
+        _want(out.lse, "out.lse", torch.float32, (R,))
+        _want(out.top_ids, "out.top_ids", torch.int32, (R, top_k))
+        _want(out.top_logprobs, "out.top_logprobs", torch.float32, (R, top_k))
+    call("mt_token_logprobs", _ptr(logits), logits.stride(0) if R > 1 else max(V, logits.stride(0)), _ptr(tokens), R,
+         V, int(top_k), _ptr(out.logprob) if tokens is not None else None, _ptr(out.entropy), _ptr(out.lse),
+         _ptr(out.top_ids), _ptr(out.top_logprobs), dtype_code(logits.dtype), _stream())
+    return out
 
 
 def device_status(clear: bool = True) -> int:
