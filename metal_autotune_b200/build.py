@@ -1,5 +1,6 @@
-"""Build libmt.so (the sm_100a region kernels) in-tree with nvcc, and
-libmt_graph.so (the host-side graph substitution engine) with g++.
+"""Build libmt.so (the sm_100a region kernels) in-tree with nvcc, and with g++
+libmt_graph.so (the host-side graph substitution engine) and mt_bind.so (the
+native Python binding of the paged-serving entry points).
 
 Each translation unit compiles with relocatable device code (the device
 status word is shared across them) and the objects are device-linked into
@@ -102,6 +103,40 @@ def build_graph_library(force: bool = False) -> Path:
     return GRAPH_LIB
 
 
+BIND_SRC = CSRC / "bind.cpp"
+BIND_LIB = LIBDIR / "mt_bind.so"
+
+
+def build_bind_library(force: bool = False) -> Path:
+    """Compile csrc/bind.cpp (a Python extension module over torch's C++
+    tensors that calls libmt.so beside it) into lib/mt_bind.so; returns its path."""
+    build_library()
+    deps = [BIND_SRC, INCLUDE / "mt.h", Path(__file__)]
+    if not force and not _stale(BIND_LIB, deps):
+        return BIND_LIB
+    import sysconfig
+
+    import torch
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("no C++ compiler; mt_bind.so cannot be built")
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+           sysconfig.get_paths()["include"]]
+    tmp = BIND_LIB.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(a for i in inc for a in ("-isystem", str(i))), str(BIND_SRC), "-o", str(tmp), f"-L{LIBDIR}", "-lmt",
+           f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {BIND_SRC.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BIND_LIB)
+    return BIND_LIB
+
+
 if __name__ == "__main__":
     print(build_library(force="--force" in sys.argv, verbose=True))
     print(build_graph_library(force="--force" in sys.argv))
+    print(build_bind_library(force="--force" in sys.argv))

@@ -1,101 +1,522 @@
 // Log-probabilities of given tokens with entropy, logsumexp and the top
-// alternatives of each row of logits.
+// alternatives of each row of logits, in one pass over the logits.
+#include <cooperative_groups.h>
+
 #include "mt_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace mt {
 namespace {
 
-constexpr int kLpThreads = 512;
-constexpr int kLpMaxTop = 32;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxTop = 32;    // one key per lane
+constexpr int kUnroll = 4;     // 16-byte loads a thread has in flight
+constexpr int kGroups = 64;    // groups of threads whose maxima bound the k-th largest value
+constexpr int kCap = 2048;     // candidates kept before the exact form takes over
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.69314718055994530942;
 
 // Larger keys first: the value's order, then the lower index. NaN sorts above
-// every number, -0 equals +0.
+// every number, -0 equals +0. No element's key is 0.
 __device__ __forceinline__ uint64_t top_key(float v, uint32_t i) {
   const uint32_t b = __float_as_uint(v + 0.0f);
   const uint32_t u = isnan(v) ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
   return static_cast<uint64_t>(u) << 32 | (0xffffffffu - i);
 }
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t u = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float((u & 0x80000000u) ? u ^ 0x80000000u : ~u);
+}
+__device__ __forceinline__ int key_index(uint64_t key) {
+  return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+
+// A 16-byte vector of logits: its maximum (NaN skipped where there is another
+// value), its values as they are, and its values with -inf raised to a finite
+// bound far below kFloor, NaN kept: 0 * -inf never arises in the sums.
+template <int DT> struct Vec;
+template <> struct Vec<MT_BF16> {
+  static constexpr int E = 8;
+  static __device__ __forceinline__ float vmax(const uint4& u) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(f.x, f.y);
+  }
+  static __device__ __forceinline__ float raw(const uint4& u, int e) {
+    return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(&u)[e]);
+  }
+  static __device__ __forceinline__ float2 pair(const uint4& u, int p) {
+    const __nv_bfloat162 low = __float2bfloat162_rn(-1e30f);
+    return __bfloat1622float2(__hmax2_nan(reinterpret_cast<const __nv_bfloat162*>(&u)[p], low));
+  }
+};
+template <> struct Vec<MT_F16> {
+  static constexpr int E = 8;
+  static __device__ __forceinline__ float vmax(const uint4& u) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(f.x, f.y);
+  }
+  static __device__ __forceinline__ float raw(const uint4& u, int e) {
+    return __half2float(reinterpret_cast<const __half*>(&u)[e]);
+  }
+  static __device__ __forceinline__ float2 pair(const uint4& u, int p) {
+    const __half2 low = __float2half2_rn(-65504.f);
+    return __half22float2(__hmax2_nan(reinterpret_cast<const __half2*>(&u)[p], low));
+  }
+};
+template <> struct Vec<MT_F32> {
+  static constexpr int E = 4;
+  static __device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+  }
+  static __device__ __forceinline__ float vmax(const uint4& u) {
+    return fmaxf(fmaxf(raw(u, 0), raw(u, 1)), fmaxf(raw(u, 2), raw(u, 3)));
+  }
+  static __device__ __forceinline__ float raw(const uint4& u, int e) {
+    return reinterpret_cast<const float*>(&u)[e];
+  }
+  static __device__ __forceinline__ float2 pair(const uint4& u, int p) {
+    return make_float2(max_nan(raw(u, 2 * p), -1e30f), max_nan(raw(u, 2 * p + 1), -1e30f));
+  }
+};
+constexpr float kFloor = -3e4f;  // rows whose maximum lies below it take the exact form
+
+// The running sums of a thread: s = sum 2^z, t = sum 2^z z, z = x log2(e) - M,
+// in two halves for the packed instructions. M is a whole number at most 1/2
+// off the largest x log2(e) seen, so z is rounded once, z of the largest value
+// is near 0, and neither sum cancels or overflows.
+struct Sums {
+  float2 s, t;
+  float M, ref;  // ref: the value M belongs to
+  __device__ __forceinline__ void raise(float v) {
+    const float m = rintf(v * kLog2e), d = M - m, f = ex2(d);
+    t.x = f * fmaf(d, s.x, t.x);
+    t.y = f * fmaf(d, s.y, t.y);
+    s.x *= f;
+    s.y *= f;
+    M = m;
+    ref = v;
+  }
+  __device__ __forceinline__ void add(float2 x) {
+    const float2 z = fma2(x, make_float2(kLog2e, kLog2e), make_float2(-M, -M));
+    const float2 p = make_float2(ex2(z.x), ex2(z.y));
+    s = add2(s, p);
+    t = fma2(p, z, t);
+  }
+};
+
+// ------------------------------------------------ a warp's sorted top 32 keys
+__device__ __forceinline__ uint64_t pick(uint64_t a, int o, bool larger) {
+  const uint64_t b = __shfl_xor_sync(0xffffffffu, a, o);
+  return (b > a) == larger ? b : a;
+}
+// bitonic sequence -> falling
+__device__ __forceinline__ uint64_t merge_down(uint64_t a, int lane) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a = pick(a, o, (lane & o) == 0);
+  return a;
+}
+// any order -> rising
+__device__ __forceinline__ uint64_t sort_up(uint64_t a, int lane) {
+#pragma unroll
+  for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+    for (int o = n >> 1; o > 0; o >>= 1) a = pick(a, o, ((lane & o) == 0) == ((lane & n) != 0 && n < 32));
+  return a;
+}
+// falling list + rising batch -> falling list of the 32 largest
+__device__ __forceinline__ uint64_t take(uint64_t list, uint64_t rising, int lane) {
+  return merge_down(list > rising ? list : rising, lane);
+}
+
+struct Slice {  // what a CTA found in its part of a row
+  double m, s, t;  // sum e^(x-m), sum e^(x-m) (x-m); s = 0 where every logit is -inf
+  uint64_t list[kMaxTop];
+};
+
+struct Smem {
+  uint64_t buf[kCap];
+  uint64_t lists[kWarps][32];
+  uint64_t group[kGroups];
+  uint64_t thr_key;
+  float first_max;
+  float red[3][kWarps];
+  double red_d[2][kWarps];
+  int count, exact;
+  Slice out;
+};
 
 struct LogprobArgs {
   const void* logits;
   int64_t stride, V;
   const int32_t* tokens;
-  int top_k;
+  int top_k, split;
   float *logprob, *entropy, *lse;
   int32_t* top_ids;
   float* top_lp;
 };
 
-// One row per CTA, three passes: maximum, sums, then top_k rounds.
+// The part of a row that one CTA reads: vectors [v0, v1) of the aligned body,
+// and, for the first part, the unaligned values before and after the body.
 template <int DT>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs a) {
-  using T = typename Elem<DT>::T;
-  __shared__ float red_f[kLpThreads / 32];
-  __shared__ double red_d[2][kLpThreads / 32];
-  __shared__ uint64_t red_k[kLpThreads / 32];
-  griddep_wait();
-  griddep_launch();
+struct Part {
+  const typename Elem<DT>::T* x;
+  int head, tail;       // values before / after the body that belong to this part
+  int64_t body, tail0;  // index of the body's first value, of the first value after it
+  int64_t v0, v1;
+  __device__ __forceinline__ const uint4* vec() const { return reinterpret_cast<const uint4*>(x + body); }
+};
+
+// Any input, several passes: every logit -inf or tiny, NaN, +inf, or more
+// candidates than the buffer holds (values that keep rising along the row).
+template <int DT>
+__device__ __noinline__ void exact_slice(Smem& sm, const Part<DT>& p, int top_k) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+  constexpr int E = Vec<DT>::E;
+  const int64_t a0 = p.body + p.v0 * E, n_body = (p.v1 - p.v0) * E;
+  const int64_t n = n_body + p.head + p.tail;
+  auto index = [&](int64_t j) {
+    return j < n_body ? a0 + j : j < n_body + p.head ? j - n_body : p.tail0 + (j - n_body - p.head);
+  };
   float m = -INFINITY;
-  for (int64_t i = tid; i < a.V; i += kLpThreads) m = fmaxf(m, Elem<DT>::to_f(x[i]));
+  for (int64_t j = tid; j < n; j += kThreads) m = fmaxf(m, Elem<DT>::to_f(p.x[index(j)]));
   m = warp_max(m);
-  if (lane == 0) red_f[warp] = m;
+  if (lane == 0) sm.red[0][warp] = m;
   __syncthreads();
-  for (int w = 0; w < kLpThreads / 32; ++w) m = fmaxf(m, red_f[w]);
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm.red[0][w]);
   double s = 0, t = 0;
-  for (int64_t i = tid; i < a.V; i += kLpThreads) {
-    const float z = Elem<DT>::to_f(x[i]) - m;
-    const float e = expf(z);
+  for (int64_t j = tid; j < n; j += kThreads) {
+    const float x = Elem<DT>::to_f(p.x[index(j)]);
+    if (x == -INFINITY) continue;
+    const float z = x - m, e = expf(z);
     s += e;
-    if (e > 0.f) t += static_cast<double>(e) * z;
+    if (e != 0.f) t += static_cast<double>(e) * z;
   }
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     s += __shfl_xor_sync(0xffffffffu, s, o);
     t += __shfl_xor_sync(0xffffffffu, t, o);
   }
   if (lane == 0) {
-    red_d[0][warp] = s;
-    red_d[1][warp] = t;
+    sm.red_d[0][warp] = s;
+    sm.red_d[1][warp] = t;
+  }
+  if (tid == 0) sm.count = 0;
+  if (tid < 32) sm.lists[0][tid] = 0;
+  __syncthreads();
+  if (tid == 0) {
+    s = t = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      s += sm.red_d[0][w];
+      t += sm.red_d[1][w];
+    }
+    sm.out.m = m;
+    sm.out.s = s;
+    sm.out.t = t;
+  }
+  if (top_k == 0) return;
+  for (int64_t j0 = 0; j0 < n; j0 += kThreads) {
+    const uint64_t least = sm.lists[0][top_k - 1];
+    if (j0 + tid < n) {
+      const int64_t i = index(j0 + tid);
+      const uint64_t key = top_key(Elem<DT>::to_f(p.x[i]), static_cast<uint32_t>(i));
+      if (key > least) sm.buf[atomicAdd(&sm.count, 1)] = key;
+    }
+    __syncthreads();
+    const int c = sm.count;  // at most kThreads
+    if (c > 0) {
+      if (warp == 0) {
+        uint64_t list = sm.lists[0][lane];
+        for (int b = 0; b < c; b += 32) list = take(list, sort_up(b + lane < c ? sm.buf[b + lane] : 0, lane), lane);
+        sm.lists[0][lane] = list;
+      }
+      __syncthreads();
+      if (tid == 0) sm.count = 0;
+    }
+    __syncthreads();
+  }
+  if (tid < 32) sm.out.list[tid] = sm.lists[0][tid];
+}
+
+// One pass. The first kUnroll vectors of every thread come in before anything
+// is decided: of the maxima of 64 groups of threads, the k-th largest bounds
+// the k-th largest logit of the slice from below, and the largest is the
+// sums' first reference. From then on a value can be among the top k only if it
+// is above that bound (an equal value later in the row ranks behind it), which
+// one comparison per vector finds out; the few that are go to a buffer in
+// shared memory and are sorted at the end. Which thread stores a candidate
+// where does not matter: keys are unique and the sort is by key.
+template <int DT>
+__device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k) {
+  using V = Vec<DT>;
+  constexpr int E = V::E;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = static_cast<int>(p.v1 - p.v0);                   // an index is below 2^31
+  const uint32_t i0 = static_cast<uint32_t>(p.body + p.v0 * E);  // index of the slice's first value
+  const uint4* v = p.vec() + p.v0;
+  uint4 r[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u)
+    if (u * kThreads + tid < n) r[u] = __ldcs(v + u * kThreads + tid);
+  // a value before or after the aligned body
+  float extra = 0.f;
+  int extra_i = -1;
+  if (tid < p.head) extra_i = tid;
+  else if (tid >= 32 && tid < 32 + p.tail) extra_i = static_cast<int>(p.tail0) + (tid - 32);
+  if (extra_i >= 0) extra = Elem<DT>::to_f(p.x[extra_i]);
+
+  uint64_t mine = 0;
+  {
+    float m = 0.f;
+    int at = -1;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (u * kThreads + tid < n) {
+        const float f = V::vmax(r[u]);
+        if (at < 0 || f > m) {
+          m = f;
+          at = u;
+        }
+      }
+    // the maximum lies in vector `at`, so at its last index or before
+    if (at >= 0) mine = top_key(m, i0 + (at * kThreads + tid) * E + E - 1);
+    // (the extra values stay out of the bound: one after the body ranks behind an equal value of the body)
+  }
+#pragma unroll
+  for (int o = 1; o < kThreads / kGroups; o <<= 1) {
+    const uint64_t k = __shfl_xor_sync(0xffffffffu, mine, o);
+    mine = k > mine ? k : mine;
+  }
+  constexpr int kPer = kThreads / kGroups;  // threads to a group, and keys each compares its group's with
+  static_assert(kPer * kPer == kGroups, "each group's threads cover all groups");
+  const int group = tid / kPer;
+  if (tid % kPer == 0) sm.group[group] = mine;
+  if (tid == 0) {
+    sm.count = 0;
+    sm.thr_key = top_k == 0 ? ~0ull : 0ull;
   }
   __syncthreads();
-  s = t = 0;
-  for (int w = 0; w < kLpThreads / 32; ++w) {
-    s += red_d[0][w];
-    t += red_d[1][w];
+  {
+    int rank = 0;  // groups ahead of this one; empty ones (key 0) by their number
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int g = (tid % kPer) * kPer + i;
+      const uint64_t k = sm.group[g];
+      rank += k > mine || (k == mine && g < group);
+    }
+#pragma unroll
+    for (int o = 1; o < kPer; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (tid % kPer == 0) {
+      if (rank == top_k - 1) sm.thr_key = mine;
+      if (rank == 0) sm.first_max = key_value(mine);
+    }
   }
-  const double lse = m + log(s);
-  if (tid == 0) {
+  __syncthreads();
+  const uint64_t thr_key = sm.thr_key;
+  const float thr = top_k == 0 ? INFINITY : key_value(thr_key);
+  Sums a;
+  a.s = a.t = make_float2(0.f, 0.f);
+  a.ref = fmaxf(sm.first_max, kFloor);
+  if (isnan(sm.first_max)) a.ref = sm.first_max;
+  a.M = rintf(a.ref * kLog2e);
+  auto push = [&](uint64_t key) {
+    const int c = atomicAdd(&sm.count, 1);
+    if (c < kCap) sm.buf[c] = key;
+  };
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u)
+    if (u * kThreads + tid < n) {
+#pragma unroll
+      for (int q = 0; q < E / 2; ++q) a.add(V::pair(r[u], q));
+      if (top_k > 0 && !(V::vmax(r[u]) < thr)) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint64_t key = top_key(V::raw(r[u], e), i0 + (u * kThreads + tid) * E + e);
+          if (key >= thr_key) push(key);
+        }
+      }
+    }
+  if (extra_i >= 0) {
+    if (extra > a.ref) a.raise(extra);
+    const float2 sv = a.s, tv = a.t;
+    a.add(make_float2(extra == -INFINITY ? -1e30f : extra, -1e30f));
+    a.s.y = sv.y;
+    a.t.y = tv.y;
+    const uint64_t key = top_key(extra, static_cast<uint32_t>(extra_i));
+    if (top_k > 0 && key >= thr_key) push(key);
+  }
+  float gate = fminf(thr, a.ref);
+  auto take_vec = [&](const uint4& w, int j) {
+    const float m = V::vmax(w);
+    if (m > gate) {
+      if (m > thr) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float f = V::raw(w, e);
+          if (f > thr) push(top_key(f, i0 + static_cast<uint32_t>(j) * E + e));
+        }
+      }
+      if (m > a.ref) {
+        a.raise(m);
+        gate = fminf(thr, m);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < E / 2; ++q) a.add(V::pair(w, q));
+  };
+  int j = kUnroll * kThreads + tid;
+  for (; j + (kUnroll - 1) * kThreads < n; j += kUnroll * kThreads) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) r[u] = __ldcs(v + j + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) take_vec(r[u], j + u * kThreads);
+  }
+  for (; j < n; j += kThreads) take_vec(__ldcs(v + j), j);
+
+  // the block's sums, relative to the largest M
+  const float mw = warp_max(a.M);
+  float d = a.M - mw, f = ex2(d);
+  float s = a.s.x + a.s.y, t = a.t.x + a.t.y;
+  t = warp_sum(f * fmaf(d, s, t));
+  s = warp_sum(f * s);
+  if (lane == 0) {
+    sm.red[0][warp] = mw;
+    sm.red[1][warp] = s;
+    sm.red[2][warp] = t;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const float mr = lane < kWarps ? sm.red[0][lane] : -INFINITY;
+    const float mb = warp_max(mr);
+    d = lane < kWarps ? mr - mb : 0.f;
+    f = lane < kWarps ? ex2(d) : 0.f;
+    s = lane < kWarps ? sm.red[1][lane] : 0.f;
+    t = lane < kWarps ? sm.red[2][lane] : 0.f;
+    t = warp_sum(f * fmaf(d, s, t));
+    s = warp_sum(f * s);
+    if (lane == 0) {
+      sm.out.m = static_cast<double>(mb) * kLn2;
+      sm.out.s = s;
+      sm.out.t = t * kLn2;
+      // the largest value alone adds 2^-1/2 at least, unless it lies below kFloor or the row holds NaN or +inf
+      sm.exact = !(s >= 0.5f && s < INFINITY && t == t) || sm.count > kCap;
+    }
+  }
+  __syncthreads();
+  if (sm.exact) return false;
+  if (top_k == 0) return true;
+  // top 32 of the candidates: batches of 32 sorted by the warps, their lists joined in pairs
+  const int c = sm.count;
+  uint64_t list = 0;
+  for (int b = warp * 32; b < c; b += kThreads) list = take(list, sort_up(b + lane < c ? sm.buf[b + lane] : 0, lane), lane);
+  int live = min(kWarps, (c + 31) >> 5);
+  while (live > 1) {
+    const int half = (live + 1) >> 1;
+    if (warp >= half && warp < live) sm.lists[warp][lane] = list;
+    __syncthreads();
+    if (warp + half < live) list = take(list, sm.lists[warp + half][31 - lane], lane);
+    live = half;
+    // a list written at the next level belongs to a warp that read, never to one that is read now
+  }
+  if (warp == 0) sm.out.list[lane] = list;
+  return true;
+}
+
+// A row per CTA, or `split` CTAs of a cluster per row where there are few rows;
+// the first joins the others' sums and lists through distributed shared memory.
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const LogprobArgs a) {
+  using T = typename Elem<DT>::T;
+  constexpr int E = Vec<DT>::E;
+  __shared__ Smem sm;
+  griddep_wait();
+  griddep_launch();
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int64_t row = blockIdx.x / a.split;
+  const int rank = static_cast<int>(blockIdx.x - row * a.split);
+  Part<DT> p;
+  p.x = static_cast<const T*>(a.logits) + row * a.stride;
+  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(p.x) & 15) / sizeof(T));
+  p.body = min(static_cast<int64_t>((E - off) % E), a.V);
+  const int64_t nvec = (a.V - p.body) / E;
+  p.tail0 = p.body + nvec * E;
+  p.v0 = nvec * rank / a.split;
+  p.v1 = nvec * (rank + 1) / a.split;
+  p.head = rank == 0 ? static_cast<int>(p.body) : 0;
+  p.tail = rank == 0 ? static_cast<int>(a.V - p.tail0) : 0;
+  if (!one_pass<DT>(sm, p, a.top_k)) exact_slice<DT>(sm, p, a.top_k);
+  __syncthreads();
+  double m = sm.out.m, s = sm.out.s, t = sm.out.t;
+  uint64_t list = tid < 32 ? sm.out.list[lane] : 0;
+  if (a.split > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (rank == 0 && tid < 32) {
+      for (int c = 1; c < a.split; ++c) {
+        const Slice* o = cluster.map_shared_rank(&sm.out, c);
+        if (a.top_k > 0) list = take(list, o->list[31 - lane], lane);
+        const double om = o->m, os = o->s, ot = o->t;
+        if (os == 0) continue;  // only -inf there
+        if (s == 0) {
+          m = om;
+          s = os;
+          t = ot;
+        } else if (om > m) {
+          const double dd = m - om, ff = exp(dd);
+          t = ot + ff * (t + dd * s);
+          s = os + ff * s;
+          m = om;
+        } else {
+          const double dd = om - m, ff = exp(dd);
+          t = t + ff * (ot + dd * os);
+          s = s + ff * os;
+        }
+      }
+    }
+    cluster.sync();  // the other CTAs' shared memory stays alive until it has been read
+    if (rank != 0) return;
+  }
+  if (tid >= 32) return;
+  const double ls = s > 0 ? log(s) : NAN, lse = m + ls;  // no distribution: NaN throughout
+  if (lane == 0) {
     if (a.lse) a.lse[row] = static_cast<float>(lse);
-    if (a.entropy) a.entropy[row] = static_cast<float>(log(s) - t / s);
+    if (a.entropy) a.entropy[row] = static_cast<float>(ls - t / s);
     if (a.tokens) {
       const int tok = a.tokens[row];
       if (tok >= a.V) report_status(0x801);
-      a.logprob[row] = tok >= 0 && tok < a.V ? static_cast<float>(Elem<DT>::to_f(x[tok]) - lse) : 0.f;
+      a.logprob[row] = tok >= 0 && tok < a.V ? static_cast<float>(Elem<DT>::to_f(p.x[tok]) - lse) : 0.f;
     }
   }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < a.top_k; ++k) {
-    uint64_t best = 0;
-    for (int64_t i = tid; i < a.V; i += kLpThreads) {
-      const uint64_t key = top_key(Elem<DT>::to_f(x[i]), static_cast<uint32_t>(i));
-      if (key < last && key > best) best = key;
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-      const uint64_t u = __shfl_xor_sync(0xffffffffu, best, o);
-      best = u > best ? u : best;
-    }
-    __syncthreads();
-    if (lane == 0) red_k[warp] = best;
-    __syncthreads();
-    for (int w = 0; w < kLpThreads / 32; ++w) best = red_k[w] > best ? red_k[w] : best;
-    last = best;
-    if (tid == 0) {
-      const uint32_t i = 0xffffffffu - static_cast<uint32_t>(best);
-      a.top_ids[row * a.top_k + k] = static_cast<int32_t>(i);
-      a.top_lp[row * a.top_k + k] = static_cast<float>(Elem<DT>::to_f(x[i]) - lse);
-    }
+  if (lane < a.top_k) {
+    a.top_ids[row * a.top_k + lane] = key_index(list);
+    a.top_lp[row * a.top_k + lane] = static_cast<float>(key_value(list) - lse);
   }
 }
 
@@ -110,8 +531,8 @@ extern "C" int mt_token_logprobs(const void* logits, int64_t row_stride, const i
   clear_error();
   MT_CHECK_ARG(R >= 0 && R < (1ll << 24) && V > 0 && V < (1ll << 31) - 1 && row_stride >= V,
                "mt_token_logprobs: R=%lld V=%lld row_stride=%lld", (long long)R, (long long)V, (long long)row_stride);
-  MT_CHECK_ARG(top_k >= 0 && top_k <= kLpMaxTop && top_k <= V, "mt_token_logprobs: top_k=%d outside 0..min(%d, V)",
-               top_k, kLpMaxTop);
+  MT_CHECK_ARG(top_k >= 0 && top_k <= kMaxTop && top_k <= V, "mt_token_logprobs: top_k=%d outside 0..min(%d, V)",
+               top_k, kMaxTop);
   if (dtype != MT_BF16 && dtype != MT_F16 && dtype != MT_F32) {
     set_error("mt_token_logprobs: unsupported dtype %d", dtype);
     return MT_ERR_UNSUPPORTED;
@@ -120,9 +541,13 @@ extern "C" int mt_token_logprobs(const void* logits, int64_t row_stride, const i
   MT_CHECK_ARG(logits && (!tokens || logprob) && (top_k == 0 || (top_ids && top_logprobs)),
                "mt_token_logprobs: null pointer");
   MT_CHECK_ARG(aligned(logits, dtype == MT_F32 ? 4 : 2), "mt_token_logprobs: logits not aligned to their type");
-  const LogprobArgs a = {logits, row_stride, V, tokens, top_k, logprob, entropy, lse, top_ids, top_logprobs};
+  int sms = 148;
+  if (int rc = device_sm_count(&sms)) return rc;
+  int split = 1;
+  while (split < 8 && R * split * 2 <= 3 * sms && V / (split * 2) >= 4096) split *= 2;
+  const LogprobArgs a = {logits, row_stride, V, tokens, top_k, split, logprob, entropy, lse, top_ids, top_logprobs};
   auto run = [&](auto kern) {
-    return launch(kern, dim3((unsigned)R), dim3(kLpThreads), 0, (cudaStream_t)stream, a);
+    return launch_cluster(kern, dim3((unsigned)(R * split)), dim3(kThreads), 0, split, (cudaStream_t)stream, a);
   };
   return dtype == MT_BF16  ? run(logprobs_kernel<MT_BF16>)
          : dtype == MT_F16 ? run(logprobs_kernel<MT_F16>)

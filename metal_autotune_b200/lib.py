@@ -549,6 +549,38 @@ def causal_conv1d(x, weight, bias=None, *, conv_state=None, silu=True, out=None)
 
 
 # ------------------------------------------------------------------ paged serving
+BIND_PATH = LIB_PATH.with_name("mt_bind.so")
+_native = None
+
+
+def native():
+    """The native binding of the paged-serving entry points (mt_bind.so): it checks the arguments,
+    allocates the outputs and calls libmt.so on the current stream. Raises FileNotFoundError if it
+    was never built."""
+    global _native
+    if _native is None:
+        load()
+        with _lock:
+            if _native is None:
+                import importlib.machinery
+                import importlib.util
+                if not BIND_PATH.exists():
+                    raise FileNotFoundError(f"{BIND_PATH} is missing: build it with `python -m metal_autotune_b200.build`")
+                loader = importlib.machinery.ExtensionFileLoader("mt_bind", str(BIND_PATH))
+                module = importlib.util.module_from_spec(importlib.util.spec_from_loader("mt_bind", loader))
+                loader.exec_module(module)
+                _native = module
+    return _native
+
+
+def _done(result, symbol: str):
+    """A native call's outputs; an entry point's error code becomes an MTError."""
+    CALLS[0] += 1
+    if type(result) is int:
+        _check(result, symbol)
+    return result
+
+
 class PagedPlan(NamedTuple):
     """One step's plan (mt_paged_plan): see `paged_plan`."""
     seq_lens: torch.Tensor
@@ -565,14 +597,6 @@ class PagedPlan(NamedTuple):
                    torch.empty(token_cap, dtype=torch.int64, device=device), i32(5))
 
 
-def _want(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple | None = None) -> torch.Tensor:
-    if t.dtype is not dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    return _dense(t, name)
-
-
 def paged_plan(ctx_lens, new_lens, block_table, free_pages, *, page_size, token_cap, free_head=None, out=None):
     """Plan one step of a batch: where its new tokens go in the paged cache.
 
@@ -581,29 +605,9 @@ def paged_plan(ctx_lens, new_lens, block_table, free_pages, *, page_size, token_
     Returns a PagedPlan (`out`, from PagedPlan.empty(B, token_cap), or a new one): seq_lens [B],
     query_start [B+1], positions / token_seq int32 and slots int64 [token_cap] (slot -1: padding or a
     refused request), counts [5] = tokens, pages wanted, pages taken, requests refused, next free_head."""
-    B = ctx_lens.shape[0]
-    i32 = torch.int32
-    _want(ctx_lens, "ctx_lens", i32, (B,))
-    _want(new_lens, "new_lens", i32, (B,))
-    _want(free_pages, "free_pages", i32)
-    if free_head is not None:
-        _want(free_head, "free_head", i32, (1,))
-    if block_table.dtype is not i32 or block_table.dim() != 2 or block_table.shape[0] != B or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"block_table must be int32 [{B}, max_pages] with contiguous rows")
-    if out is None:
-        out = PagedPlan.empty(B, token_cap, ctx_lens.device)
-    else:
-        for t, name, dt, n in zip(out, PagedPlan._fields, (i32, i32, i32, i32, torch.int64, i32),
-                                  (B, B + 1, token_cap, token_cap, token_cap, 5)):
-            _want(t, f"out.{name}", dt, (n,))
-    width = block_table.shape[1]
-    call("mt_paged_plan", _ptr(ctx_lens), _ptr(new_lens), B, _ptr(block_table),
-         block_table.stride(0) if B > 1 else max(width, block_table.stride(0)), width, _ptr(free_pages),
-         free_pages.numel(), _ptr(free_head), int(page_size), int(token_cap), _ptr(out.seq_lens),
-         _ptr(out.query_start), _ptr(out.positions), _ptr(out.token_seq), _ptr(out.slots), _ptr(out.counts),
-         _stream())
-    return out
+    r = _done((_native or native()).paged_plan(ctx_lens, new_lens, block_table, free_pages, page_size, token_cap, free_head,
+                                               out), "mt_paged_plan")
+    return r if out is not None else PagedPlan._make(r)
 
 
 def rope_frequencies(dims, *, base=10000.0, scaling=None, device="cuda"):
@@ -648,15 +652,6 @@ def rope_frequencies(dims, *, base=10000.0, scaling=None, device="cuda"):
     return torch.tensor(freqs, dtype=torch.float32, device=device), mscale
 
 
-def _check_cache(k_cache, v_cache, dtype):
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
-        raise ValueError("k_cache and v_cache must be [pages, Hkv, page_size, D] of one shape and strides")
-    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
-        raise TypeError(f"the caches must be {dtype}, as q")
-    if k_cache.stride(3) != 1:
-        raise ValueError("the caches' rows (D) must be contiguous")
-
-
 def rope_paged_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq, *, traditional=False, mscale=1.0,
                       q_norm_w=None, k_norm_w=None, eps=1e-6, out=None, k_out=None):
     """Optional q/k RMSNorm, rotary embedding of the first 2*len(inv_freq) values of each head at
@@ -666,33 +661,19 @@ def rope_paged_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq, *, 
     projection's rows); positions int32 [T], slots int64 [T] (negative: not written); caches
     [pages, Hkv, page_size, D] (or a permuted view of that shape). Returns the rotated q, dense
     [T, Hq, D] or `out` (which may be q). `k_out` dense [T, Hkv, D] also receives the rotated k."""
-    T, Hq, D = q.shape
-    Hkv = k.shape[1]
-    dt = q.dtype
-    if k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D) or k.dtype is not dt or v.dtype is not dt:
-        raise ValueError(f"k and v must be {dt} [{T}, Hkv, {D}]")
-    if q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1:
-        raise ValueError("q, k and v must have D contiguous")
-    _check_cache(k_cache, v_cache, dt)
-    if k_cache.shape[1] != Hkv or k_cache.shape[3] != D:
-        raise ValueError(f"the caches must be [pages, {Hkv}, page_size, {D}]")
-    _want(positions, "positions", torch.int32, (T,))
-    _want(slots, "slots", torch.int64, (T,))
-    _want(inv_freq, "inv_freq", torch.float32)
-    for w, name in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
-        if w is not None:
-            _want(w, name, dt, (D,))
-    y = out if out is not None else torch.empty((T, Hq, D), dtype=dt, device=q.device)
-    if y is not q and (y.shape != q.shape or y.dtype is not dt or y.stride(2) != 1):
-        raise ValueError("out must have q's shape and dtype with D contiguous")
-    if k_out is not None:
-        _want(k_out, "k_out", dt, (T, Hkv, D))
-    call("mt_rope_paged_append", _ptr(q), _ptr(k), _ptr(v), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-         v.stride(0), v.stride(1), _ptr(q_norm_w), _ptr(k_norm_w), float(eps), _ptr(positions), _ptr(slots),
-         _ptr(inv_freq), 2 * inv_freq.shape[0], int(bool(traditional)), float(mscale), _ptr(y), y.stride(0),
-         y.stride(1), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], k_cache.shape[2],
-         k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), T, Hq, Hkv, D, dtype_code(dt), _stream())
-    return y
+    return _done((_native or native()).rope_paged_append(q, k, v, positions, slots, k_cache, v_cache, inv_freq, traditional,
+                                                         mscale, q_norm_w, k_norm_w, eps, out, k_out),
+                 "mt_rope_paged_append")
+
+
+_paged_ws: dict[int, int] = {}
+
+
+def paged_sdpa_decode_workspace_bytes(D: int) -> int:
+    n = _paged_ws.get(D)
+    if n is None:
+        n = _paged_ws[D] = int(load().mt_paged_sdpa_decode_workspace_bytes(D))
+    return n
 
 
 def paged_sdpa_decode(q, k_cache, v_cache, block_table, seq_lens, *, scale, out=None, workspace=None):
@@ -700,38 +681,9 @@ def paged_sdpa_decode(q, k_cache, v_cache, block_table, seq_lens, *, scale, out=
     page_size, D] (or a permuted view of that shape), block_table int32 [B, max_pages], seq_lens int32
     [B] (0: that request's output is zeros). Returns [B, Hq, D]. `workspace`: a Workspace of the
     caller's own, for calls on a stream other than the one that uses the device's shared workspace."""
-    B, Hq, D = q.shape
-    dt = q.dtype
-    _check_cache(k_cache, v_cache, dt)
-    pages, Hkv, page_size, _ = k_cache.shape
-    if k_cache.shape[3] != D:
-        raise ValueError(f"the caches must be [pages, Hkv, page_size, {D}]")
-    if q.stride(2) != 1:
-        raise ValueError("q must have D contiguous")
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"block_table must be int32 [{B}, max_pages] with contiguous rows")
-    _want(seq_lens, "seq_lens", torch.int32, (B,))
-    o = out if out is not None else torch.empty((B, Hq, D), dtype=dt, device=q.device)
-    if o.shape != q.shape or o.dtype is not dt or o.stride(2) != 1:
-        raise ValueError("out must have q's shape and dtype with D contiguous")
-    ws = workspace if workspace is not None else Workspace.get(_paged_ws_bytes(D))
-    width = block_table.shape[1]
-    call("mt_paged_sdpa_decode", _ptr(q), q.stride(0), q.stride(1), _ptr(k_cache), _ptr(v_cache), pages, page_size,
-         k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), _ptr(block_table),
-         block_table.stride(0) if B > 1 else max(width, block_table.stride(0)), width, _ptr(seq_lens), _ptr(o),
-         o.stride(0), o.stride(1), B, Hq, Hkv, D, float(scale), dtype_code(dt), ws.ptr, ws.nbytes, _stream())
-    return o
-
-
-_paged_ws: dict[int, int] = {}
-
-
-def _paged_ws_bytes(D: int) -> int:
-    n = _paged_ws.get(D)
-    if n is None:
-        n = _paged_ws[D] = int(load().mt_paged_sdpa_decode_workspace_bytes(D))
-    return n
+    ws = workspace if workspace is not None else Workspace.get(paged_sdpa_decode_workspace_bytes(q.shape[-1]))
+    return _done((_native or native()).paged_sdpa_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out, ws.buf),
+                 "mt_paged_sdpa_decode")
 
 
 class TokenLogprobs(NamedTuple):
@@ -754,24 +706,8 @@ def token_logprobs(logits, tokens=None, *, top_k=0, out=None):
     entropy, logsumexp and top_k alternatives (ids and log-probabilities in falling order, ties to the
     lower id). tokens int32 [R] (negative: 0) or None; fp32 results in a TokenLogprobs (`out`, from
     TokenLogprobs.empty(R, top_k), or a new one)."""
-    if logits.dim() != 2 or logits.stride(1) != 1:
-        raise ValueError("logits must be [R, V] with contiguous rows")
-    R, V = logits.shape
-    if tokens is not None:
-        _want(tokens, "tokens", torch.int32, (R,))
-    if out is None:
-        out = TokenLogprobs.empty(R, top_k, logits.device, tokens is not None)
-    else:
-        if tokens is not None:
-            _want(out.logprob, "out.logprob", torch.float32, (R,))
-        _want(out.entropy, "out.entropy", torch.float32, (R,))
-        _want(out.lse, "out.lse", torch.float32, (R,))
-        _want(out.top_ids, "out.top_ids", torch.int32, (R, top_k))
-        _want(out.top_logprobs, "out.top_logprobs", torch.float32, (R, top_k))
-    call("mt_token_logprobs", _ptr(logits), logits.stride(0) if R > 1 else max(V, logits.stride(0)), _ptr(tokens), R,
-         V, int(top_k), _ptr(out.logprob) if tokens is not None else None, _ptr(out.entropy), _ptr(out.lse),
-         _ptr(out.top_ids), _ptr(out.top_logprobs), dtype_code(logits.dtype), _stream())
-    return out
+    r = _done((_native or native()).token_logprobs(logits, tokens, top_k, out), "mt_token_logprobs")
+    return r if out is not None else TokenLogprobs._make(r)
 
 
 def device_status(clear: bool = True) -> int:

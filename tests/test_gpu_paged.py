@@ -390,7 +390,7 @@ def test_attend_on_a_stream_of_its_own(cuda):
     q, kc, vc, table, ln = attend_case([3000, 5, 900], 8, 2, 128, 16, "bf16", seed=6)
     want = lib.paged_sdpa_decode(q, kc, vc, table, ln, scale=0.1)
     torch.cuda.synchronize()
-    side, ws = torch.cuda.Stream(), lib.Workspace(torch.cuda.current_device(), lib._paged_ws_bytes(128))
+    side, ws = torch.cuda.Stream(), lib.Workspace(torch.cuda.current_device(), lib.paged_sdpa_decode_workspace_bytes(128))
     torch.cuda.synchronize()
     with torch.cuda.stream(side):
         got = [lib.paged_sdpa_decode(q, kc, vc, table, ln, scale=0.1, workspace=ws) for _ in range(20)]

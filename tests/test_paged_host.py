@@ -105,8 +105,12 @@ def test_logprobs_refuses(mt):
     assert logprobs(R=0, x=None) == 0
 
 
-def test_wrappers_check_their_tensors():
+def test_wrappers_check_their_tensors(monkeypatch):
     """Shape and type errors come from the wrappers, by name, before any pointer is taken."""
+    build.build_bind_library()
+    cpu_workspace = lib.Workspace.__new__(lib.Workspace)
+    cpu_workspace.buf = torch.zeros(16, dtype=torch.uint8)
+    monkeypatch.setattr(lib.Workspace, "get", classmethod(lambda cls, n: cpu_workspace))
     z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)  # noqa: E731
     i = lambda *s: z(*s, dt=torch.int32)  # noqa: E731
     with pytest.raises(ValueError, match="new_lens must have shape"):
