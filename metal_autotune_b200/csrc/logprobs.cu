@@ -9,11 +9,18 @@ namespace cg = cooperative_groups;
 namespace mt {
 namespace {
 
-constexpr int kThreads = 512;
+// 5 CTAs of 256 threads per SM, 64 bytes in flight a thread: 2048 x 151936 bf16 with 20 alternatives 126 us; 4 CTAs
+// 133, 6 (40 registers, spilled) 165, 3 vectors in flight 133, 3 CTAs of 512 threads 142.
+constexpr int kThreads = 256;
+constexpr int kCtasPerSm = 5;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;    // one key per lane
-constexpr int kUnroll = 4;     // 16-byte loads a thread has in flight
+constexpr int kMaxSplit = 8;   // CTAs to a row
+static_assert(kMaxSplit <= kWarps, "the first CTA joins a list per warp");
+constexpr int kUnroll = 4;     // 16-byte loads a thread has in flight (a batch)
+constexpr int kBatch = kThreads * kUnroll;
 constexpr int kGroups = 64;    // groups of threads whose maxima bound the k-th largest value
+constexpr int kEntries = 32;   // maxima of its batches that a thread keeps
 constexpr int kCap = 2048;     // candidates kept before the exact form takes over
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
@@ -165,12 +172,26 @@ struct Smem {
   uint64_t lists[kWarps][32];
   uint64_t group[kGroups];
   uint64_t thr_key;
-  float first_max;
+  __nv_bfloat16 batch_max[kEntries][kThreads];
   float red[3][kWarps];
   double red_d[2][kWarps];
-  int count, exact;
+  int count, hits, exact;
   Slice out;
 };
+
+// The top 32 keys of the first `live` warps' falling lists, in warp 0, joined
+// in pairs. All threads take part.
+__device__ __forceinline__ uint64_t join_lists(Smem& sm, uint64_t list, int live) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  while (live > 1) {
+    const int half = (live + 1) >> 1;
+    if (warp >= half && warp < live) sm.lists[warp][lane] = list;
+    __syncthreads();
+    if (warp + half < live) list = take(list, sm.lists[warp + half][31 - lane], lane);
+    live = half;  // the lists written next belong to warps that read here, none is read twice
+  }
+  return list;
+}
 
 struct LogprobArgs {
   const void* logits;
@@ -265,14 +286,16 @@ __device__ __noinline__ void exact_slice(Smem& sm, const Part<DT>& p, int top_k)
   if (tid < 32) sm.out.list[tid] = sm.lists[0][tid];
 }
 
-// One pass. The first kUnroll vectors of every thread come in before anything
-// is decided: of the maxima of 64 groups of threads, the k-th largest bounds
-// the k-th largest logit of the slice from below, and the largest is the
-// sums' first reference. From then on a value can be among the top k only if it
-// is above that bound (an equal value later in the row ranks behind it), which
-// one comparison per vector finds out; the few that are go to a buffer in
-// shared memory and are sorted at the end. Which thread stores a candidate
-// where does not matter: keys are unique and the sort is by key.
+// One pass over the logits for the sums, with a note of where large values are:
+// each thread keeps the maximum of every batch of 4 vectors that it read (in
+// bf16, rounded up) and its largest value. Of the maxima of 64 groups of
+// threads, the k-th largest bounds the k-th largest logit from below, at about
+// 1.2 k values above it for logits in no particular order; only batches that
+// reach the bound are read a second time, and their values that do are sorted.
+// An equal value counts up to the bound's own place in the row (ties go to the
+// lower index), so constant or masked stretches stay within the buffer too.
+// Which thread stores a candidate where does not matter: keys are unique and
+// the sort is by key.
 template <int DT>
 __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k) {
   using V = Vec<DT>;
@@ -281,124 +304,89 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
   const int n = static_cast<int>(p.v1 - p.v0);                   // an index is below 2^31
   const uint32_t i0 = static_cast<uint32_t>(p.body + p.v0 * E);  // index of the slice's first value
   const uint4* v = p.vec() + p.v0;
-  uint4 r[kUnroll];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u)
-    if (u * kThreads + tid < n) r[u] = __ldcs(v + u * kThreads + tid);
-  // a value before or after the aligned body
+  const int batches = (n + kBatch - 1) / kBatch;
+  const int per = (batches + kEntries - 1) / kEntries;  // batches to an entry
+  uint4 none;                                           // -inf throughout
+  none.x = none.y = none.z = none.w = DT == MT_BF16 ? 0xff80ff80u : DT == MT_F16 ? 0xfc00fc00u : 0xff800000u;
+
+  Sums a;
+  a.s = a.t = make_float2(0.f, 0.f);
+  a.ref = kFloor;
+  a.M = rintf(kFloor * kLog2e);
+  // a value before or after the aligned body; it stays out of the bound (one after the body ranks behind its equals)
   float extra = 0.f;
   int extra_i = -1;
   if (tid < p.head) extra_i = tid;
   else if (tid >= 32 && tid < 32 + p.tail) extra_i = static_cast<int>(p.tail0) + (tid - 32);
-  if (extra_i >= 0) extra = Elem<DT>::to_f(p.x[extra_i]);
-
-  uint64_t mine = 0;
-  {
-    float m = 0.f;
-    int at = -1;
+  if (extra_i >= 0) {
+    extra = Elem<DT>::to_f(p.x[extra_i]);
+    if (extra > a.ref) a.raise(extra);
+    a.add(make_float2(extra == -INFINITY ? -1e30f : extra, -1e30f));
+    a.s.y = a.t.y = 0.f;
+  }
+  float top = 0.f;  // the thread's largest value, in vector `at` (the first that holds it)
+  int at = -1, entry = 0, in_entry = 0;
+  auto take_batch = [&](const uint4 (&r)[kUnroll], int j0) {
+    float m[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) m[u] = V::vmax(r[u]);
+    float mb = m[0];
+#pragma unroll
+    for (int u = 1; u < kUnroll; ++u) mb = fmaxf(mb, m[u]);
+    if (top_k > 0) {
+      if (at < 0 || mb > top) {
+        top = mb;
+        int first = kUnroll - 1;
+#pragma unroll
+        for (int u = kUnroll - 2; u >= 0; --u) first = m[u] == mb ? u : first;
+        at = j0 + first * kThreads;
+      }
+      __nv_bfloat16 up = __float2bfloat16_ru(mb);
+      if (in_entry > 0) up = __hmax(up, sm.batch_max[entry][tid]);
+      sm.batch_max[entry][tid] = up;
+      if (++in_entry == per) {
+        in_entry = 0;
+        ++entry;
+      }
+    }
+    if (mb > a.ref + 1.0f) a.raise(mb);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (u * kThreads + tid < n) {
-        const float f = V::vmax(r[u]);
-        if (at < 0 || f > m) {
-          m = f;
-          at = u;
-        }
-      }
-    // the maximum lies in vector `at`, so at its last index or before
-    if (at >= 0) mine = top_key(m, i0 + (at * kThreads + tid) * E + E - 1);
-    // (the extra values stay out of the bound: one after the body ranks behind an equal value of the body)
+#pragma unroll
+      for (int q = 0; q < E / 2; ++q) a.add(V::pair(r[u], q));
+  };
+  int j0 = 0;
+  for (; j0 + kBatch <= n; j0 += kBatch) {
+    uint4 r[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) r[u] = __ldcs(v + j0 + u * kThreads + tid);
+    take_batch(r, j0);
   }
+  if (j0 < n) {
+    uint4 r[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int j = j0 + u * kThreads + tid;
+      r[u] = j < n ? __ldcs(v + j) : none;
+    }
+    take_batch(r, j0);
+  }
+
+  // the bound: the k-th largest of the groups' maxima
+  uint64_t mine = 0;
+  if (tid < n && top_k > 0) mine = top_key(top, i0 + static_cast<uint32_t>(at + tid) * E + E - 1);
 #pragma unroll
   for (int o = 1; o < kThreads / kGroups; o <<= 1) {
     const uint64_t k = __shfl_xor_sync(0xffffffffu, mine, o);
     mine = k > mine ? k : mine;
   }
-  constexpr int kPer = kThreads / kGroups;  // threads to a group, and keys each compares its group's with
-  static_assert(kPer * kPer == kGroups, "each group's threads cover all groups");
+  constexpr int kPer = kThreads / kGroups;  // threads to a group; together they compare its key with all groups'
   const int group = tid / kPer;
   if (tid % kPer == 0) sm.group[group] = mine;
   if (tid == 0) {
-    sm.count = 0;
-    sm.thr_key = top_k == 0 ? ~0ull : 0ull;
+    sm.count = sm.hits = 0;
+    sm.thr_key = 0;
   }
-  __syncthreads();
-  {
-    int rank = 0;  // groups ahead of this one; empty ones (key 0) by their number
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int g = (tid % kPer) * kPer + i;
-      const uint64_t k = sm.group[g];
-      rank += k > mine || (k == mine && g < group);
-    }
-#pragma unroll
-    for (int o = 1; o < kPer; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-    if (tid % kPer == 0) {
-      if (rank == top_k - 1) sm.thr_key = mine;
-      if (rank == 0) sm.first_max = key_value(mine);
-    }
-  }
-  __syncthreads();
-  const uint64_t thr_key = sm.thr_key;
-  const float thr = top_k == 0 ? INFINITY : key_value(thr_key);
-  Sums a;
-  a.s = a.t = make_float2(0.f, 0.f);
-  a.ref = fmaxf(sm.first_max, kFloor);
-  if (isnan(sm.first_max)) a.ref = sm.first_max;
-  a.M = rintf(a.ref * kLog2e);
-  auto push = [&](uint64_t key) {
-    const int c = atomicAdd(&sm.count, 1);
-    if (c < kCap) sm.buf[c] = key;
-  };
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u)
-    if (u * kThreads + tid < n) {
-#pragma unroll
-      for (int q = 0; q < E / 2; ++q) a.add(V::pair(r[u], q));
-      if (top_k > 0 && !(V::vmax(r[u]) < thr)) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint64_t key = top_key(V::raw(r[u], e), i0 + (u * kThreads + tid) * E + e);
-          if (key >= thr_key) push(key);
-        }
-      }
-    }
-  if (extra_i >= 0) {
-    if (extra > a.ref) a.raise(extra);
-    const float2 sv = a.s, tv = a.t;
-    a.add(make_float2(extra == -INFINITY ? -1e30f : extra, -1e30f));
-    a.s.y = sv.y;
-    a.t.y = tv.y;
-    const uint64_t key = top_key(extra, static_cast<uint32_t>(extra_i));
-    if (top_k > 0 && key >= thr_key) push(key);
-  }
-  float gate = fminf(thr, a.ref);
-  auto take_vec = [&](const uint4& w, int j) {
-    const float m = V::vmax(w);
-    if (m > gate) {
-      if (m > thr) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float f = V::raw(w, e);
-          if (f > thr) push(top_key(f, i0 + static_cast<uint32_t>(j) * E + e));
-        }
-      }
-      if (m > a.ref) {
-        a.raise(m);
-        gate = fminf(thr, m);
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < E / 2; ++q) a.add(V::pair(w, q));
-  };
-  int j = kUnroll * kThreads + tid;
-  for (; j + (kUnroll - 1) * kThreads < n; j += kUnroll * kThreads) {
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) r[u] = __ldcs(v + j + u * kThreads);
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) take_vec(r[u], j + u * kThreads);
-  }
-  for (; j < n; j += kThreads) take_vec(__ldcs(v + j), j);
 
   // the block's sums, relative to the largest M
   const float mw = warp_max(a.M);
@@ -412,6 +400,18 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
     sm.red[2][warp] = t;
   }
   __syncthreads();
+  {
+    int rank = 0;  // groups ahead of this one; empty ones (key 0) by their number
+#pragma unroll
+    for (int i = 0; i < kGroups / kPer; ++i) {
+      const int g = i * kPer + tid % kPer;
+      const uint64_t k = sm.group[g];
+      rank += k > mine || (k == mine && g < group);
+    }
+#pragma unroll
+    for (int o = 1; o < kPer; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (tid % kPer == 0 && rank == top_k - 1) sm.thr_key = mine;
+  }
   if (warp == 0) {
     const float mr = lane < kWarps ? sm.red[0][lane] : -INFINITY;
     const float mb = warp_max(mr);
@@ -425,26 +425,54 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
       sm.out.m = static_cast<double>(mb) * kLn2;
       sm.out.s = s;
       sm.out.t = t * kLn2;
-      // the largest value alone adds 2^-1/2 at least, unless it lies below kFloor or the row holds NaN or +inf
-      sm.exact = !(s >= 0.5f && s < INFINITY && t == t) || sm.count > kCap;
+      // the largest value alone adds over 1/2, unless it lies below kFloor or the row holds NaN or +inf
+      sm.exact = !(s >= 0.25f && s < INFINITY && t == t);
     }
   }
   __syncthreads();
   if (sm.exact) return false;
   if (top_k == 0) return true;
+  const uint64_t thr_key = sm.thr_key;
+  const float thr = key_value(thr_key);  // NaN where fewer than k groups hold anything: all count
+  auto push = [&](uint64_t key) {
+    if (key < thr_key) return;
+    const int c = atomicAdd(&sm.count, 1);
+    if (c < kCap) sm.buf[c] = key;
+  };
+  auto look = [&](int j) {
+    const uint4 w = v[j];
+    if (V::vmax(w) < thr) return;
+#pragma unroll
+    for (int i = 0; i < E; ++i) push(top_key(V::raw(w, i), i0 + static_cast<uint32_t>(j) * E + i));
+  };
+  // the batches that reach the bound, as their first vectors; read again by all threads at once
+  int* hits = reinterpret_cast<int*>(sm.lists);
+  constexpr int kHits = sizeof(sm.lists) / sizeof(int);
+  const int span = per * kBatch;
+  for (int e = 0; e * span < n; ++e)
+    if (!(__bfloat162float(sm.batch_max[e][tid]) < thr)) {
+      const int h = atomicAdd(&sm.hits, 1);
+      if (h < kHits) hits[h] = e * span + tid;
+    }
+  __syncthreads();
+  if (sm.hits <= kHits) {
+    for (int i = tid; i < sm.hits * per * kUnroll; i += kThreads) {
+      const int h = i / (per * kUnroll), j = hits[h] + (i - h * per * kUnroll) * kThreads;
+      if (j < n) look(j);
+    }
+  } else {  // long stretches of equal values
+    for (int e = 0; e * span < n; ++e)
+      if (!(__bfloat162float(sm.batch_max[e][tid]) < thr))
+        for (int j = e * span + tid; j < min(n, (e + 1) * span); j += kThreads) look(j);
+  }
+  if (extra_i >= 0) push(top_key(extra, static_cast<uint32_t>(extra_i)));
+  __syncthreads();
+  if (sm.count > kCap) return false;
   // top 32 of the candidates: batches of 32 sorted by the warps, their lists joined in pairs
   const int c = sm.count;
   uint64_t list = 0;
   for (int b = warp * 32; b < c; b += kThreads) list = take(list, sort_up(b + lane < c ? sm.buf[b + lane] : 0, lane), lane);
-  int live = min(kWarps, (c + 31) >> 5);
-  while (live > 1) {
-    const int half = (live + 1) >> 1;
-    if (warp >= half && warp < live) sm.lists[warp][lane] = list;
-    __syncthreads();
-    if (warp + half < live) list = take(list, sm.lists[warp + half][31 - lane], lane);
-    live = half;
-    // a list written at the next level belongs to a warp that read, never to one that is read now
-  }
+  list = join_lists(sm, list, min(kWarps, (c + 31) >> 5));
   if (warp == 0) sm.out.list[lane] = list;
   return true;
 }
@@ -452,10 +480,11 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
 // A row per CTA, or `split` CTAs of a cluster per row where there are few rows;
 // the first joins the others' sums and lists through distributed shared memory.
 template <int DT>
-__global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const LogprobArgs a) {
   using T = typename Elem<DT>::T;
   constexpr int E = Vec<DT>::E;
-  __shared__ Smem sm;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   griddep_wait();
   griddep_launch();
   const int tid = threadIdx.x, lane = tid & 31;
@@ -478,25 +507,26 @@ __global__ void __launch_bounds__(kThreads, 3) logprobs_kernel(const LogprobArgs
   if (a.split > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    if (rank == 0 && tid < 32) {
-      for (int c = 1; c < a.split; ++c) {
-        const Slice* o = cluster.map_shared_rank(&sm.out, c);
-        if (a.top_k > 0) list = take(list, o->list[31 - lane], lane);
-        const double om = o->m, os = o->s, ot = o->t;
-        if (os == 0) continue;  // only -inf there
-        if (s == 0) {
-          m = om;
-          s = os;
-          t = ot;
-        } else if (om > m) {
-          const double dd = m - om, ff = exp(dd);
-          t = ot + ff * (t + dd * s);
-          s = os + ff * s;
-          m = om;
-        } else {
-          const double dd = om - m, ff = exp(dd);
-          t = t + ff * (ot + dd * os);
-          s = s + ff * os;
+    if (rank == 0) {
+      const int warp = tid >> 5;
+      if (a.top_k > 0) {  // a list per warp
+        if (warp < a.split) list = cluster.map_shared_rank(&sm.out, warp)->list[lane];
+        list = join_lists(sm, list, a.split);
+      }
+      if (warp == 0) {  // sums, a slice per lane of each eight
+        const int c = lane & (kMaxSplit - 1);
+        const Slice* o = cluster.map_shared_rank(&sm.out, c < a.split ? c : 0);
+        const double om = o->m, os = c < a.split ? o->s : 0.0, ot = o->t;
+        m = os == 0 ? -INFINITY : om;  // a slice of -inf alone, or a lane without one
+#pragma unroll
+        for (int q = kMaxSplit / 2; q > 0; q >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, q));
+        const double f = exp(om - m);
+        s = os == 0 ? 0.0 : f * os;
+        t = os == 0 ? 0.0 : f * (ot + (om - m) * os);
+#pragma unroll
+        for (int q = kMaxSplit / 2; q > 0; q >>= 1) {
+          s += __shfl_xor_sync(0xffffffffu, s, q);
+          t += __shfl_xor_sync(0xffffffffu, t, q);
         }
       }
     }
@@ -544,10 +574,11 @@ extern "C" int mt_token_logprobs(const void* logits, int64_t row_stride, const i
   int sms = 148;
   if (int rc = device_sm_count(&sms)) return rc;
   int split = 1;
-  while (split < 8 && R * split * 2 <= 3 * sms && V / (split * 2) >= 4096) split *= 2;
+  while (split < kMaxSplit && R * split * 2 <= kCtasPerSm * sms && V / (split * 2) >= 4096) split *= 2;
   const LogprobArgs a = {logits, row_stride, V, tokens, top_k, split, logprob, entropy, lse, top_ids, top_logprobs};
-  auto run = [&](auto kern) {
-    return launch_cluster(kern, dim3((unsigned)(R * split)), dim3(kThreads), 0, split, (cudaStream_t)stream, a);
+  auto run = [&](auto kern) -> int {
+    if (int e = ensure_smem(kern, sizeof(Smem))) return e;
+    return launch_cluster(kern, dim3((unsigned)(R * split)), dim3(kThreads), sizeof(Smem), split, (cudaStream_t)stream, a);
   };
   return dtype == MT_BF16  ? run(logprobs_kernel<MT_BF16>)
          : dtype == MT_F16 ? run(logprobs_kernel<MT_F16>)

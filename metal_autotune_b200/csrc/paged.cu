@@ -254,14 +254,194 @@ __device__ __forceinline__ void store8(typename Elem<DT>::T* p, const float (&x)
 
 constexpr int kAppendThreads = 256;
 
-// One token (or one of `splits` parts of its rows) per CTA: the angles of its
-// position once in shared memory, then each row of 8-element lanes, LPR lanes
-// to a row (8, 16 or 32 for heads of up to 64, 128, 256). The angle is reduced
-// to a fraction of a turn in double, so a position of 2^20 rotates as exactly
-// as position 1; norm and rotation stay in fp32 and are rounded once, on the
-// way out.
+// cos and sin (times mscale) of the token's angles, each once, in shared
+// memory. The angle is reduced to a fraction of a turn in double, so a position
+// of 2^30 rotates as exactly as position 1.
+__device__ __forceinline__ void angles(const AppendArgs& a, int64_t t, float2* turn) {
+  for (int j = threadIdx.x; j < a.dims >> 1; j += kAppendThreads) {
+    const double turns = static_cast<double>(a.positions[t]) * static_cast<double>(a.inv_freq[j]) * 0.15915494309189533577;
+    float s, c;
+    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+    turn[j] = make_float2(c * a.mscale, s * a.mscale);
+  }
+}
+
+// offset of the token's cache row (without the head), -1 where it has none
+__device__ __forceinline__ int64_t slot_offset(const AppendArgs& a, int64_t t) {
+  const int64_t slot = a.slots[t];
+  if (slot < 0) return -1;
+  const int64_t page = slot < (1ll << 31) ? static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.page_size))
+                                           : slot / a.page_size;
+  if (page < a.num_pages) return page * a.page_stride + (slot - page * a.page_size) * a.slot_stride;
+  report_status(0x701);
+  return -1;
+}
+
+// 4 consecutive elements as they are in memory
+template <int DT> struct Quad;
+template <> struct Quad<MT_BF16> { using U = uint2; };
+template <> struct Quad<MT_F16> { using U = uint2; };
+template <> struct Quad<MT_F32> { using U = float4; };
+template <int DT>
+__device__ __forceinline__ void unpack4(const typename Quad<DT>::U& u, float* x) {
+  if constexpr (DT == MT_F32) {
+    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+  } else {
+    const typename Elem<DT>::T2* e = reinterpret_cast<const typename Elem<DT>::T2*>(&u);
+    const float2 a = Elem<DT>::unpack2(e[0]), b = Elem<DT>::unpack2(e[1]);
+    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+  }
+}
+template <int DT>
+__device__ __forceinline__ typename Quad<DT>::U pack4(const float* x) {
+  if constexpr (DT == MT_F32) {
+    return make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    typename Quad<DT>::U u;
+    typename Elem<DT>::T2* e = reinterpret_cast<typename Elem<DT>::T2*>(&u);
+    e[0] = Elem<DT>::pack2(x[0], x[1]);
+    e[1] = Elem<DT>::pack2(x[2], x[3]);
+    return u;
+  }
+}
+
+// One token (or one of `splits` parts of its rows) per CTA, LPR lanes to a row
+// (8, 16 or 32 for heads of up to 64, 128, 256), for `dims` in whole eights. A
+// lane holds two pieces of four values that rotate with each other: (j, j +
+// dims/2), or eight adjacent ones; past `dims`, eight that are copied. So its
+// four angles and its norm weights stay in registers for all rows, no value
+// crosses lanes but the norm's sum, and the rows' loads are under way before
+// the position is known. Norm and rotation in fp32, rounded once.
+#ifndef AP_ROWS
+#define AP_ROWS 3
+#define AP_MIN 3
+#endif
+template <int DT, int LPR, bool TRAD, bool NORM, int ROWS>
+__global__ void __launch_bounds__(kAppendThreads, ROWS > 1 ? AP_MIN : 2) append_kernel(const AppendArgs a) {
+  using T = typename Elem<DT>::T;
+  using Q = typename Quad<DT>::U;
+  constexpr int kRows = kAppendThreads / LPR;
+  __shared__ __align__(16) float2 turn[128];
+  __shared__ int64_t dst;
+  griddep_wait();
+  griddep_launch();
+  const int tid = threadIdx.x;
+  const int64_t t = blockIdx.x / a.splits;
+  const int part = blockIdx.x - static_cast<int>(t) * a.splits;
+  const int half = a.dims >> 1, sub = tid % LPR;
+  const bool in = sub * 8 < a.D, turned = sub * 8 < a.dims;
+  // the lane's two pieces of a row
+  const int pa = !in ? 0 : TRAD || !turned ? sub * 8 : sub * 4;
+  const int pb = !in ? 0 : TRAD || !turned ? sub * 8 + 4 : half + sub * 4;
+  const int H = a.Hq + 2 * a.Hkv;
+  const T* q = static_cast<const T*>(a.q) + t * a.q_st;
+  const T* k = static_cast<const T*>(a.k) + t * a.k_st;
+  const T* v = static_cast<const T*>(a.v) + t * a.v_st;
+  Q ra[ROWS], rb[ROWS];
+  int row = part * kRows + tid / LPR;
+  auto load = [&]() {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = row + i * a.splits * kRows;
+      if (r < H && in) {
+        const T* src = r < a.Hq ? q + r * a.q_sh : r < a.Hq + a.Hkv ? k + (r - a.Hq) * a.k_sh : v + (r - a.Hq - a.Hkv) * a.v_sh;
+        ra[i] = *reinterpret_cast<const Q*>(src + pa);
+        rb[i] = *reinterpret_cast<const Q*>(src + pb);
+      }
+    }
+  };
+  load();
+  Q wq[2], wk[2];
+  if constexpr (NORM) {
+    if (a.q_w) {
+      wq[0] = *reinterpret_cast<const Q*>(static_cast<const T*>(a.q_w) + pa);
+      wq[1] = *reinterpret_cast<const Q*>(static_cast<const T*>(a.q_w) + pb);
+    }
+    if (a.k_w) {
+      wk[0] = *reinterpret_cast<const Q*>(static_cast<const T*>(a.k_w) + pa);
+      wk[1] = *reinterpret_cast<const Q*>(static_cast<const T*>(a.k_w) + pb);
+    }
+  }
+  angles(a, t, turn);
+  if (tid == kAppendThreads - 1) dst = slot_offset(a, t);
+  __syncthreads();
+  const int64_t off = dst;
+  float2 cs[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) cs[i] = in && turned ? turn[sub * 4 + i] : make_float2(1.f, 0.f);
+  while (true) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = row + i * a.splits * kRows;
+      const bool live = r < H && in;
+      const bool is_q = r < a.Hq, is_v = r >= a.Hq + a.Hkv;
+      const int h = is_q ? r : is_v ? r - a.Hq - a.Hkv : r - a.Hq;
+      Q oa = ra[i], ob = rb[i];
+      float x[8];
+      if (live) {
+        unpack4<DT>(ra[i], x);
+        unpack4<DT>(rb[i], x + 4);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+      }
+      if constexpr (NORM) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (!is_v && (is_q ? a.q_w : a.k_w)) {
+          const float g = 1.0f / sqrtf(ss / static_cast<float>(a.D) + a.eps);
+          float w[8];
+          unpack4<DT>(is_q ? wq[0] : wk[0], w);
+          unpack4<DT>(is_q ? wq[1] : wk[1], w + 4);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= g * w[e];
+        }
+      }
+      if (!live) continue;
+      if (!is_v) {
+        float y[8];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int i0 = TRAD ? 2 * p : p, i1 = TRAD ? 2 * p + 1 : p + 4;
+          y[i0] = x[i0] * cs[p].x - x[i1] * cs[p].y;
+          y[i1] = x[i1] * cs[p].x + x[i0] * cs[p].y;
+        }
+        if (!turned) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = x[e];
+        }
+        oa = pack4<DT>(y);
+        ob = pack4<DT>(y + 4);
+      }
+      T* to = nullptr;
+      if (is_q) {
+        to = static_cast<T*>(a.q_out) + t * a.qo_st + h * a.qo_sh;
+      } else {
+        if (!is_v && a.k_out) {
+          T* ko = static_cast<T*>(a.k_out) + (t * a.Hkv + h) * a.D;
+          *reinterpret_cast<Q*>(ko + pa) = oa;
+          *reinterpret_cast<Q*>(ko + pb) = ob;
+        }
+        if (off >= 0) to = static_cast<T*>(is_v ? a.v_cache : a.k_cache) + off + h * a.head_stride;
+      }
+      if (to) {
+        *reinterpret_cast<Q*>(to + pa) = oa;
+        *reinterpret_cast<Q*>(to + pb) = ob;
+      }
+    }
+    row += ROWS * a.splits * kRows;
+    if (__all_sync(0xffffffffu, row >= H)) break;
+    load();
+  }
+}
+
+// `dims` not a multiple of 8: a lane's values rotate with others anywhere in
+// the row, fetched one by one. Such heads are rare and small.
 template <int DT, int LPR, bool TRAD>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads) append_any_kernel(const AppendArgs a) {
   using T = typename Elem<DT>::T;
   constexpr int kRows = kAppendThreads / LPR;
   __shared__ float2 turn[128];
@@ -272,22 +452,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   const int64_t t = blockIdx.x / a.splits;
   const int part = blockIdx.x % a.splits;
   const int half = a.dims >> 1;
-  for (int j = tid; j < half; j += kAppendThreads) {
-    const double turns = static_cast<double>(a.positions[t]) * static_cast<double>(a.inv_freq[j]) * 0.15915494309189533577;
-    float s, c;
-    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
-    turn[j] = make_float2(c * a.mscale, s * a.mscale);
-  }
-  if (tid == kAppendThreads - 1) {
-    const int64_t slot = a.slots[t];
-    int64_t off = -1;
-    if (slot >= 0) {
-      const int64_t page = slot / a.page_size;
-      if (page < a.num_pages) off = page * a.page_stride + (slot - page * a.page_size) * a.slot_stride;
-      else report_status(0x701);
-    }
-    dst = off;
-  }
+  angles(a, t, turn);
+  if (tid == kAppendThreads - 1) dst = slot_offset(a, t);
   __syncthreads();
   const int64_t off = dst;
   const int sub = tid % LPR, e0 = sub * 8;
@@ -440,11 +606,17 @@ int mt_rope_paged_append(const void* q, const void* k, const void* v, int64_t q_
   if (T < sms * 4) a.splits = (int)parts;
   const dim3 grid(static_cast<unsigned>(T * a.splits));
   auto run = [&](auto kern) { return launch(kern, grid, dim3(kAppendThreads), 0, (cudaStream_t)stream, a); };
-#define MT_APPEND(DT)                                                                                       \
-  (lpr == 8    ? (traditional ? run(append_kernel<DT, 8, true>) : run(append_kernel<DT, 8, false>))         \
-   : lpr == 16 ? (traditional ? run(append_kernel<DT, 16, true>) : run(append_kernel<DT, 16, false>))       \
-               : (traditional ? run(append_kernel<DT, 32, true>) : run(append_kernel<DT, 32, false>)))
+  const bool norm = q_norm_w != nullptr || k_norm_w != nullptr;
+// one row per lane group where the rows are spread over CTAs, else three under way at once
+#define MT_APPEND_K(DT, L, TR, N) (a.splits > 1 ? run(append_kernel<DT, L, TR, N, 1>) : run(append_kernel<DT, L, TR, N, AP_ROWS>))
+#define MT_APPEND_L(DT, L)                                                                                      \
+  (dims % 8 != 0 ? (traditional ? run(append_any_kernel<DT, L, true>) : run(append_any_kernel<DT, L, false>))   \
+   : traditional ? (norm ? MT_APPEND_K(DT, L, true, true) : MT_APPEND_K(DT, L, true, false))                    \
+                 : (norm ? MT_APPEND_K(DT, L, false, true) : MT_APPEND_K(DT, L, false, false)))
+#define MT_APPEND(DT) (lpr == 8 ? MT_APPEND_L(DT, 8) : lpr == 16 ? MT_APPEND_L(DT, 16) : MT_APPEND_L(DT, 32))
   return dtype == MT_BF16 ? MT_APPEND(MT_BF16) : dtype == MT_F16 ? MT_APPEND(MT_F16) : MT_APPEND(MT_F32);
+#undef MT_APPEND_K
+#undef MT_APPEND_L
 #undef MT_APPEND
 }
 
