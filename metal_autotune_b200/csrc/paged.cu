@@ -216,7 +216,8 @@ struct AppendArgs {
   int64_t num_pages, page_stride, head_stride, slot_stride;
   int page_size;
   int Hq, Hkv, D;
-  int splits;  // CTAs per token
+  int splits;  // items per token
+  int64_t T;
 };
 
 // 8 consecutive elements of a row as fp32
@@ -252,23 +253,24 @@ __device__ __forceinline__ void store8(typename Elem<DT>::T* p, const float (&x)
   }
 }
 
-constexpr int kAppendThreads = 256;
+// Three rows to a group of lanes, two stages, 6 CTAs of 128 threads per SM (80 registers, 24 KB of ring each): 8192
+// tokens of 32/8 heads of 128 in 39.6 us. 5 CTAs with three stages 42.5; 7 or 8, whose registers spill, 58 and 62.
+constexpr int kAppendRows = 3;
+constexpr int kAppendStages = 2;
+constexpr int kAppendCtas = 6;
+constexpr int kAppendThreads = 128;
 
-// cos and sin (times mscale) of the token's angles, each once, in shared
-// memory. The angle is reduced to a fraction of a turn in double, so a position
-// of 2^30 rotates as exactly as position 1.
-__device__ __forceinline__ void angles(const AppendArgs& a, int64_t t, float2* turn) {
-  for (int j = threadIdx.x; j < a.dims >> 1; j += kAppendThreads) {
-    const double turns = static_cast<double>(a.positions[t]) * static_cast<double>(a.inv_freq[j]) * 0.15915494309189533577;
-    float s, c;
-    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
-    turn[j] = make_float2(c * a.mscale, s * a.mscale);
-  }
+// cos and sin (times mscale) of one angle. The angle is reduced to a fraction
+// of a turn in double, so a position of 2^30 rotates as exactly as position 1.
+__device__ __forceinline__ float2 cos_sin(int pos, float inv_freq, float mscale) {
+  const double turns = static_cast<double>(pos) * static_cast<double>(inv_freq) * 0.15915494309189533577;
+  float s, c;
+  sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+  return make_float2(c * mscale, s * mscale);
 }
 
 // offset of the token's cache row (without the head), -1 where it has none
-__device__ __forceinline__ int64_t slot_offset(const AppendArgs& a, int64_t t) {
-  const int64_t slot = a.slots[t];
+__device__ __forceinline__ int64_t slot_offset(const AppendArgs& a, int64_t slot) {
   if (slot < 0) return -1;
   const int64_t page = slot < (1ll << 31) ? static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.page_size))
                                            : slot / a.page_size;
@@ -277,168 +279,228 @@ __device__ __forceinline__ int64_t slot_offset(const AppendArgs& a, int64_t t) {
   return -1;
 }
 
-// 4 consecutive elements as they are in memory
-template <int DT> struct Quad;
-template <> struct Quad<MT_BF16> { using U = uint2; };
-template <> struct Quad<MT_F16> { using U = uint2; };
-template <> struct Quad<MT_F32> { using U = float4; };
-template <int DT>
-__device__ __forceinline__ void unpack4(const typename Quad<DT>::U& u, float* x) {
-  if constexpr (DT == MT_F32) {
-    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-  } else {
-    const typename Elem<DT>::T2* e = reinterpret_cast<const typename Elem<DT>::T2*>(&u);
-    const float2 a = Elem<DT>::unpack2(e[0]), b = Elem<DT>::unpack2(e[1]);
-    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
-  }
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
 }
-template <int DT>
-__device__ __forceinline__ typename Quad<DT>::U pack4(const float* x) {
-  if constexpr (DT == MT_F32) {
-    return make_float4(x[0], x[1], x[2], x[3]);
-  } else {
-    typename Quad<DT>::U u;
-    typename Elem<DT>::T2* e = reinterpret_cast<typename Elem<DT>::T2*>(&u);
-    e[0] = Elem<DT>::pack2(x[0], x[1]);
-    e[1] = Elem<DT>::pack2(x[2], x[3]);
-    return u;
-  }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
 }
 
-// One token (or one of `splits` parts of its rows) per CTA, LPR lanes to a row
-// (8, 16 or 32 for heads of up to 64, 128, 256), for `dims` in whole eights. A
-// lane holds two pieces of four values that rotate with each other: (j, j +
-// dims/2), or eight adjacent ones; past `dims`, eight that are copied. So its
-// four angles and its norm weights stay in registers for all rows, no value
-// crosses lanes but the norm's sum, and the rows' loads are under way before
-// the position is known. Norm and rotation in fp32, rounded once.
-#ifndef AP_ROWS
-#define AP_ROWS 3
-#define AP_MIN 3
-#endif
-template <int DT, int LPR, bool TRAD, bool NORM, int ROWS>
-__global__ void __launch_bounds__(kAppendThreads, ROWS > 1 ? AP_MIN : 2) append_kernel(const AppendArgs a) {
+// the 16 bytes of a piece of a row as pairs of fp32, and back with one rounding
+template <int DT>
+__device__ __forceinline__ void unpack(const uint4& u, float2* x) {
+  if constexpr (DT == MT_F32) {
+    x[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    x[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  } else {
+    const typename Elem<DT>::T2* e = reinterpret_cast<const typename Elem<DT>::T2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = Elem<DT>::unpack2(e[i]);
+  }
+}
+template <int DT>
+__device__ __forceinline__ uint4 pack(const float2* x) {
+  uint4 u;
+  if constexpr (DT == MT_F32) {
+    u = make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x), __float_as_uint(x[1].y));
+  } else {
+    typename Elem<DT>::T2* e = reinterpret_cast<typename Elem<DT>::T2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = Elem<DT>::pack2(x[i].x, x[i].y);
+  }
+  return u;
+}
+
+// An item is a token's rows, or as many of them as a CTA takes at a time: ROWS
+// to each group of LPR lanes. A lane holds two 16-byte pieces of a row whose
+// values rotate with each other: (j, j + dims/2), or adjacent ones; past
+// `dims`, two that are copied. No value crosses lanes but the norm's sum, and a
+// thread reads back only what it copied to shared memory itself: the rows of
+// the next STAGES - 1 items are always under way and need no barrier. The
+// angles of the next item are worked out, one by a thread, while this one's
+// rows arrive; one barrier per item hands them over. What limits it is
+// instructions, not memory: so two fp32 values to an instruction, and rows'
+// addresses, angles and weights come out of shared memory, which leaves
+// registers for six CTAs to an SM.
+template <int DT, int LPR, bool TRAD, int ROWS, int STAGES>
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(const AppendArgs a) {
   using T = typename Elem<DT>::T;
-  using Q = typename Quad<DT>::U;
-  constexpr int kRows = kAppendThreads / LPR;
-  __shared__ __align__(16) float2 turn[128];
-  __shared__ int64_t dst;
+  constexpr int P = 16 / sizeof(T);  // values to a piece
+  constexpr int kRows = kAppendThreads / LPR, kGroup = ROWS * kRows;
+  struct Row {
+    const T* src;  // token 0's row, and the way from token to token
+    int64_t st;
+    T* to;     // where it goes, but for the token's offset in q_out or its slot's in the cache
+    int kind;  // 0 q, 1 k, 2 v, -1 no row
+    int head;
+  };
+  extern __shared__ __align__(16) uint8_t append_smem[];
+  uint4(*ring)[ROWS][2][kAppendThreads] = reinterpret_cast<uint4(*)[ROWS][2][kAppendThreads]>(append_smem);
+  __shared__ __align__(16) float cos_of[2][128], sin_of[2][128], neg_sin_of[2][128];
+  __shared__ __align__(16) T weight[2][256];
+  __shared__ __align__(16) Row rows[kGroup];
+  __shared__ int64_t dst[2];
   griddep_wait();
   griddep_launch();
   const int tid = threadIdx.x;
-  const int64_t t = blockIdx.x / a.splits;
-  const int part = blockIdx.x - static_cast<int>(t) * a.splits;
   const int half = a.dims >> 1, sub = tid % LPR;
-  const bool in = sub * 8 < a.D, turned = sub * 8 < a.dims;
+  const bool in = sub * 2 * P < a.D, turned = sub * 2 * P < a.dims;
   // the lane's two pieces of a row
-  const int pa = !in ? 0 : TRAD || !turned ? sub * 8 : sub * 4;
-  const int pb = !in ? 0 : TRAD || !turned ? sub * 8 + 4 : half + sub * 4;
-  const int H = a.Hq + 2 * a.Hkv;
-  const T* q = static_cast<const T*>(a.q) + t * a.q_st;
-  const T* k = static_cast<const T*>(a.k) + t * a.k_st;
-  const T* v = static_cast<const T*>(a.v) + t * a.v_st;
-  Q ra[ROWS], rb[ROWS];
-  int row = part * kRows + tid / LPR;
-  auto load = [&]() {
+  const int pa = !in ? 0 : TRAD || !turned ? sub * 2 * P : sub * P;
+  const int pb = !in ? 0 : TRAD || !turned ? sub * 2 * P + P : half + sub * P;
+  // the grid is a multiple of `splits`: this CTA's part of the rows, its first token and the way to the next
+  const int part = blockIdx.x % a.splits;
+  const int64_t step = gridDim.x / a.splits;
+  int64_t t = blockIdx.x / a.splits;
+  // position and slot of the next token, for the threads that use them
+  const bool has_angle = tid < half, has_slot = tid == kAppendThreads - 1;
+  const float inv = has_angle ? a.inv_freq[tid] : 0.f;
+  int pos = has_angle ? a.positions[t] : 0;
+  int64_t slot = has_slot ? a.slots[t] : -1;
+  const bool norm_q = a.q_w != nullptr, norm_k = a.k_w != nullptr;
+  for (int i = tid; i < kGroup; i += kAppendThreads) {
+    const int r = part * kGroup + i;
+    Row w = {nullptr, 0, nullptr, -1, 0};
+    if (r < a.Hq)
+      w = {static_cast<const T*>(a.q) + r * a.q_sh, a.q_st, static_cast<T*>(a.q_out) + r * a.qo_sh, 0, r};
+    else if (r < a.Hq + a.Hkv)
+      w = {static_cast<const T*>(a.k) + (r - a.Hq) * a.k_sh, a.k_st,
+           static_cast<T*>(a.k_cache) + (r - a.Hq) * a.head_stride, 1, r - a.Hq};
+    else if (r < a.Hq + 2 * a.Hkv)
+      w = {static_cast<const T*>(a.v) + (r - a.Hq - a.Hkv) * a.v_sh, a.v_st,
+           static_cast<T*>(a.v_cache) + (r - a.Hq - a.Hkv) * a.head_stride, 2, r - a.Hq - a.Hkv};
+    rows[i] = w;
+  }
+  for (int i = tid; i < a.D; i += kAppendThreads) {
+    if (norm_q) weight[0][i] = static_cast<const T*>(a.q_w)[i];
+    if (norm_k) weight[1][i] = static_cast<const T*>(a.k_w)[i];
+  }
+  __syncthreads();
+  int64_t ahead = t;  // the token whose rows are fetched next
+  auto issue = [&](int stage) {
+    if (ahead < a.T && in) {
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const int r = row + i * a.splits * kRows;
-      if (r < H && in) {
-        const T* src = r < a.Hq ? q + r * a.q_sh : r < a.Hq + a.Hkv ? k + (r - a.Hq) * a.k_sh : v + (r - a.Hq - a.Hkv) * a.v_sh;
-        ra[i] = *reinterpret_cast<const Q*>(src + pa);
-        rb[i] = *reinterpret_cast<const Q*>(src + pb);
+      for (int i = 0; i < ROWS; ++i) {
+        const Row& w = rows[i * kRows + tid / LPR];
+        if (w.src) {
+          const T* src = w.src + ahead * w.st;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(&ring[stage][i][0][tid])), "l"(src + pa) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(&ring[stage][i][1][tid])), "l"(src + pb) : "memory");
+        }
       }
+    }
+    ahead += step;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) issue(s);
+  const float inv_d = 1.0f / static_cast<float>(a.D);
+  auto hand_over = [&](int buf, int64_t next) {  // the angles of the token that pos and slot are of; then the next one's
+    if (has_angle) {
+      const float2 cs = cos_sin(pos, inv, a.mscale);
+      cos_of[buf][tid] = cs.x;
+      sin_of[buf][tid] = cs.y;
+      neg_sin_of[buf][tid] = -cs.y;
+    }
+    if (has_slot) dst[buf] = slot_offset(a, slot);
+    if (next < a.T) {
+      if (has_angle) pos = a.positions[next];
+      if (has_slot) slot = a.slots[next];
     }
   };
-  load();
-  Q wq[2], wk[2];
-  if constexpr (NORM) {
-    if (a.q_w) {
-      wq[0] = *reinterpret_cast<const Q*>(static_cast<const T*>(a.q_w) + pa);
-      wq[1] = *reinterpret_cast<const Q*>(static_cast<const T*>(a.q_w) + pb);
-    }
-    if (a.k_w) {
-      wk[0] = *reinterpret_cast<const Q*>(static_cast<const T*>(a.k_w) + pa);
-      wk[1] = *reinterpret_cast<const Q*>(static_cast<const T*>(a.k_w) + pb);
-    }
-  }
-  angles(a, t, turn);
-  if (tid == kAppendThreads - 1) dst = slot_offset(a, t);
+  hand_over(0, t + step);
   __syncthreads();
-  const int64_t off = dst;
-  float2 cs[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) cs[i] = in && turned ? turn[sub * 4 + i] : make_float2(1.f, 0.f);
-  while (true) {
+  int buf = 0, get = 0, put = STAGES - 1;
+  for (; t < a.T; t += step) {
+    issue(put);
+    put = put + 1 == STAGES ? 0 : put + 1;
+    if (t + step < a.T) hand_over(buf ^ 1, t + 2 * step);
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    const int64_t off = dst[buf], q_off = t * a.qo_st;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const int r = row + i * a.splits * kRows;
-      const bool live = r < H && in;
-      const bool is_q = r < a.Hq, is_v = r >= a.Hq + a.Hkv;
-      const int h = is_q ? r : is_v ? r - a.Hq - a.Hkv : r - a.Hq;
-      Q oa = ra[i], ob = rb[i];
-      float x[8];
-      if (live) {
-        unpack4<DT>(ra[i], x);
-        unpack4<DT>(rb[i], x + 4);
-      } else {
+      const Row& w = rows[i * kRows + tid / LPR];
+      const int kind = w.kind;
+      uint4 oa = ring[get][i][0][tid], ob = ring[get][i][1][tid];  // (where there is no row, whatever is there)
+      if (__any_sync(0xffffffffu, kind == 0 || kind == 1)) {
+        float2 x[P / 2], y[P / 2];
+        unpack<DT>(oa, x);
+        unpack<DT>(ob, y);
+        if (norm_q || norm_k) {
+          float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.f;
-      }
-      if constexpr (NORM) {
-        float ss = 0.f;
+          for (int e = 0; e < P / 2; ++e) ss = fma2(y[e], y[e], fma2(x[e], x[e], ss));
+          float sum = in ? ss.x + ss.y : 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+          for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (kind == 1 ? norm_k : norm_q) {
+            const float g = rsqrtf(fmaf(sum, inv_d, a.eps));
+            const float2 gg = make_float2(g, g);
+            const T* ws = weight[kind == 1];
+            float2 wf[P / 2];
+            unpack<DT>(*reinterpret_cast<const uint4*>(ws + pa), wf);
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (!is_v && (is_q ? a.q_w : a.k_w)) {
-          const float g = 1.0f / sqrtf(ss / static_cast<float>(a.D) + a.eps);
-          float w[8];
-          unpack4<DT>(is_q ? wq[0] : wk[0], w);
-          unpack4<DT>(is_q ? wq[1] : wk[1], w + 4);
+            for (int e = 0; e < P / 2; ++e) x[e] = mul2(x[e], mul2(wf[e], gg));
+            unpack<DT>(*reinterpret_cast<const uint4*>(ws + pb), wf);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= g * w[e];
+            for (int e = 0; e < P / 2; ++e) y[e] = mul2(y[e], mul2(wf[e], gg));
+          }
+        }
+        if (turned) {
+          const float2* c = reinterpret_cast<const float2*>(&cos_of[buf][sub * P]);
+          const float2* s = reinterpret_cast<const float2*>(&sin_of[buf][sub * P]);
+          if constexpr (TRAD) {  // pairs within a piece: angles 0.. of the lane in x, then in y
+#pragma unroll
+            for (int e = 0; e < P / 2; ++e) {
+              const float2 c0 = c[e / 2], s0 = s[e / 2], c1 = c[(P / 2 + e) / 2], s1 = s[(P / 2 + e) / 2];
+              const float cx = (e & 1) ? c0.y : c0.x, sx = (e & 1) ? s0.y : s0.x;
+              const float cy = (e & 1) ? c1.y : c1.x, sy = (e & 1) ? s1.y : s1.x;
+              x[e] = make_float2(x[e].x * cx - x[e].y * sx, x[e].y * cx + x[e].x * sx);
+              y[e] = make_float2(y[e].x * cy - y[e].y * sy, y[e].y * cy + y[e].x * sy);
+            }
+          } else {
+            const float2* ns = reinterpret_cast<const float2*>(&neg_sin_of[buf][sub * P]);
+#pragma unroll
+            for (int e = 0; e < P / 2; ++e) {
+              const float2 u = x[e], v = y[e];
+              x[e] = fma2(u, c[e], mul2(v, ns[e]));
+              y[e] = fma2(v, c[e], mul2(u, s[e]));
+            }
+          }
+        }
+        if (kind < 2) {
+          oa = pack<DT>(x);
+          ob = pack<DT>(y);
         }
       }
-      if (!live) continue;
-      if (!is_v) {
-        float y[8];
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const int i0 = TRAD ? 2 * p : p, i1 = TRAD ? 2 * p + 1 : p + 4;
-          y[i0] = x[i0] * cs[p].x - x[i1] * cs[p].y;
-          y[i1] = x[i1] * cs[p].x + x[i0] * cs[p].y;
-        }
-        if (!turned) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = x[e];
-        }
-        oa = pack4<DT>(y);
-        ob = pack4<DT>(y + 4);
+      if (!in || kind < 0) continue;
+      if (kind == 1 && a.k_out) {
+        T* ko = static_cast<T*>(a.k_out) + (t * a.Hkv + w.head) * a.D;
+        *reinterpret_cast<uint4*>(ko + pa) = oa;
+        *reinterpret_cast<uint4*>(ko + pb) = ob;
       }
-      T* to = nullptr;
-      if (is_q) {
-        to = static_cast<T*>(a.q_out) + t * a.qo_st + h * a.qo_sh;
-      } else {
-        if (!is_v && a.k_out) {
-          T* ko = static_cast<T*>(a.k_out) + (t * a.Hkv + h) * a.D;
-          *reinterpret_cast<Q*>(ko + pa) = oa;
-          *reinterpret_cast<Q*>(ko + pb) = ob;
-        }
-        if (off >= 0) to = static_cast<T*>(is_v ? a.v_cache : a.k_cache) + off + h * a.head_stride;
-      }
-      if (to) {
-        *reinterpret_cast<Q*>(to + pa) = oa;
-        *reinterpret_cast<Q*>(to + pb) = ob;
+      if (kind == 0 || off >= 0) {
+        T* d = w.to + (kind == 0 ? q_off : off);
+        *reinterpret_cast<uint4*>(d + pa) = oa;
+        *reinterpret_cast<uint4*>(d + pb) = ob;
       }
     }
-    row += ROWS * a.splits * kRows;
-    if (__all_sync(0xffffffffu, row >= H)) break;
-    load();
+    get = get + 1 == STAGES ? 0 : get + 1;
+    buf ^= 1;
+    __syncthreads();
   }
 }
 
-// `dims` not a multiple of 8: a lane's values rotate with others anywhere in
+// `dims` or the head not in whole pieces: a lane's values rotate with others anywhere in
 // the row, fetched one by one. Such heads are rare and small.
 template <int DT, int LPR, bool TRAD>
 __global__ void __launch_bounds__(kAppendThreads) append_any_kernel(const AppendArgs a) {
@@ -452,8 +514,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_any_kernel(const Append
   const int64_t t = blockIdx.x / a.splits;
   const int part = blockIdx.x % a.splits;
   const int half = a.dims >> 1;
-  angles(a, t, turn);
-  if (tid == kAppendThreads - 1) dst = slot_offset(a, t);
+  if (tid < half) turn[tid] = cos_sin(a.positions[t], a.inv_freq[tid], a.mscale);
+  if (tid == kAppendThreads - 1) dst = slot_offset(a, a.slots[t]);
   __syncthreads();
   const int64_t off = dst;
   const int sub = tid % LPR, e0 = sub * 8;
@@ -598,26 +660,42 @@ int mt_rope_paged_append(const void* q, const void* k, const void* v, int64_t q_
                "mt_rope_paged_append: rows must be 16-byte aligned, strides multiples of 8 elements");
   AppendArgs a = {q, k, v, q_st, q_sh, k_st, k_sh, v_st, v_sh, q_norm_w, k_norm_w, eps, mscale, positions, slots,
                   inv_freq, dims, q_out, qo_st, qo_sh, k_out, k_cache, v_cache, num_pages, page_stride, head_stride,
-                  slot_stride, (int)page_size, (int)Hq, (int)Hkv, (int)D, 1};
-  const int lpr = D <= 64 ? 8 : D <= 128 ? 16 : 32;
+                  slot_stride, (int)page_size, (int)Hq, (int)Hkv, (int)D, 1, T};
   int sms = 148;
   if (int rc = device_sm_count(&sms)) return rc;
-  const int64_t parts = (Hq + 2 * Hkv + kAppendThreads / lpr - 1) / (kAppendThreads / lpr);
-  if (T < sms * 4) a.splits = (int)parts;
-  const dim3 grid(static_cast<unsigned>(T * a.splits));
-  auto run = [&](auto kern) { return launch(kern, grid, dim3(kAppendThreads), 0, (cudaStream_t)stream, a); };
-  const bool norm = q_norm_w != nullptr || k_norm_w != nullptr;
-// one row per lane group where the rows are spread over CTAs, else three under way at once
-#define MT_APPEND_K(DT, L, TR, N) (a.splits > 1 ? run(append_kernel<DT, L, TR, N, 1>) : run(append_kernel<DT, L, TR, N, AP_ROWS>))
-#define MT_APPEND_L(DT, L)                                                                                      \
-  (dims % 8 != 0 ? (traditional ? run(append_any_kernel<DT, L, true>) : run(append_any_kernel<DT, L, false>))   \
-   : traditional ? (norm ? MT_APPEND_K(DT, L, true, true) : MT_APPEND_K(DT, L, true, false))                    \
-                 : (norm ? MT_APPEND_K(DT, L, false, true) : MT_APPEND_K(DT, L, false, false)))
-#define MT_APPEND(DT) (lpr == 8 ? MT_APPEND_L(DT, 8) : lpr == 16 ? MT_APPEND_L(DT, 16) : MT_APPEND_L(DT, 32))
-  return dtype == MT_BF16 ? MT_APPEND(MT_BF16) : dtype == MT_F16 ? MT_APPEND(MT_F16) : MT_APPEND(MT_F32);
-#undef MT_APPEND_K
+  const int64_t rows = Hq + 2 * Hkv;
+  const int piece = dtype == MT_F32 ? 4 : 8;
+  const bool pieces = dims % (2 * piece) == 0 && D % (2 * piece) == 0;
+  int lpr = pieces && piece == 8 ? 4 : 8;  // lanes to a row: whole pairs of pieces, or eights
+  while (lpr * (pieces ? 2 * piece : 8) < D) lpr *= 2;
+  const int per_pass = kAppendThreads / lpr;
+  // few tokens: one row to a group of lanes, spread over as many CTAs; else three to a group
+  const bool few = T * ((rows + per_pass - 1) / per_pass) <= sms * kAppendCtas;
+  const int per_cta = pieces ? per_pass * (few ? 1 : kAppendRows) : few ? per_pass : 1 << 20;
+  a.splits = (int)((rows + per_cta - 1) / per_cta);
+  int64_t grid = T * a.splits;
+  auto run = [&](auto kern, size_t smem) -> int {
+    if (int e = ensure_smem(kern, smem)) return e;
+    return launch(kern, dim3((unsigned)grid), dim3(kAppendThreads), smem, (cudaStream_t)stream, a);
+  };
+  if (pieces && grid > sms * kAppendCtas) grid = sms * kAppendCtas < a.splits ? a.splits : sms * kAppendCtas / a.splits * a.splits;
+#define MT_APPEND_K(DT, L, TR)                                                              \
+  (few ? run(append_kernel<DT, L, TR, 1, 2>, sizeof(uint4) * 2 * kAppendThreads * 2)        \
+       : run(append_kernel<DT, L, TR, kAppendRows, kAppendStages>, sizeof(uint4) * 2 * kAppendThreads * kAppendRows * kAppendStages))
+#define MT_APPEND_L(DT, L) (traditional ? MT_APPEND_K(DT, L, true) : MT_APPEND_K(DT, L, false))
+#define MT_APPEND_ANY(DT, L) (traditional ? run(append_any_kernel<DT, L, true>, 0) : run(append_any_kernel<DT, L, false>, 0))
+#define MT_APPEND_16(DT)                                                                     \
+  (!pieces ? (lpr == 8 ? MT_APPEND_ANY(DT, 8) : lpr == 16 ? MT_APPEND_ANY(DT, 16) : MT_APPEND_ANY(DT, 32)) \
+           : lpr == 4 ? MT_APPEND_L(DT, 4) : lpr == 8 ? MT_APPEND_L(DT, 8) : MT_APPEND_L(DT, 16))
+#define MT_APPEND_32(DT)                                                                     \
+  (!pieces ? (lpr == 8 ? MT_APPEND_ANY(DT, 8) : lpr == 16 ? MT_APPEND_ANY(DT, 16) : MT_APPEND_ANY(DT, 32)) \
+           : lpr <= 8 ? MT_APPEND_L(DT, 8) : lpr == 16 ? MT_APPEND_L(DT, 16) : MT_APPEND_L(DT, 32))
+  return dtype == MT_BF16 ? MT_APPEND_16(MT_BF16) : dtype == MT_F16 ? MT_APPEND_16(MT_F16) : MT_APPEND_32(MT_F32);
+#undef MT_APPEND_32
+#undef MT_APPEND_16
+#undef MT_APPEND_ANY
 #undef MT_APPEND_L
-#undef MT_APPEND
+#undef MT_APPEND_K
 }
 
 }  // extern "C"
