@@ -110,6 +110,24 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType dt, int dev) {
   return at::detail::empty_cuda(shape, dt, c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(dev)), std::nullopt);
 }
 
+// Several outputs in one allocation, each at a multiple of 16 bytes: an
+// allocation of its own costs each of them about a microsecond.
+struct Outputs {
+  at::Tensor base;
+  int64_t at = 0;
+  static int64_t room(int64_t n, size_t size) { return (n * static_cast<int64_t>(size) + 15) & ~int64_t{15}; }
+  Outputs(int64_t bytes, int dev) : base(empty({bytes}, at::kByte, dev)) {}
+  at::Tensor take(at::IntArrayRef shape, at::ScalarType dt) {
+    const size_t size = c10::elementSize(dt);
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(),
+                                                            c10::scalarTypeToTypeMeta(dt));
+    t.unsafeGetTensorImpl()->set_storage_offset(at / static_cast<int64_t>(size));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    at += room(t.numel(), size);
+    return t;
+  }
+};
+
 template <typename T = void>
 T* ptr(const at::Tensor* t) {
   return t ? static_cast<T*>(t->data_ptr()) : nullptr;
@@ -190,9 +208,12 @@ PyObject* paged_plan(PyObject* const* a) {
       want(o[i], names[i], i == 4 ? at::kLong : at::kInt, {sizes[i]});
     }
   const int dev = on_device({&ctx, &fresh, &table, &pages, head});
-  if (a[7] == Py_None)
-    for (int i = 0; i < 6; ++i) o[i] = empty({sizes[i]}, i == 4 ? at::kLong : at::kInt, dev);
-  else
+  if (a[7] == Py_None) {
+    int64_t bytes = 0;
+    for (int i = 0; i < 6; ++i) bytes += Outputs::room(sizes[i], i == 4 ? 8 : 4);
+    Outputs out(bytes, dev);
+    for (int i = 0; i < 6; ++i) o[i] = out.take({sizes[i]}, i == 4 ? at::kLong : at::kInt);
+  } else
     on_device({&o[0], &o[1], &o[2], &o[3], &o[4], &o[5]});
   const int rc = mt_paged_plan(ptr<int32_t>(ctx), ptr<int32_t>(fresh), B, ptr<int32_t>(table), tb.stride, tb.width,
                                ptr<int32_t>(pages), pages.numel(), ptr<int32_t>(head), page_size, cap, ptr<int32_t>(o[0]),
@@ -295,11 +316,12 @@ PyObject* token_logprobs(PyObject* const* a) {
   if (a[3] != Py_None) {
     on_device({tokens ? &lp : nullptr, &entropy, &lse, &ids, &top});
   } else {
-    if (tokens) lp = empty({R}, at::kFloat, dev);
-    entropy = empty({R}, at::kFloat, dev);
-    lse = empty({R}, at::kFloat, dev);
-    ids = empty({R, k}, at::kInt, dev);
-    top = empty({R, k}, at::kFloat, dev);
+    Outputs out((tokens ? 3 : 2) * Outputs::room(R, 4) + 2 * Outputs::room(R * k, 4), dev);
+    if (tokens) lp = out.take({R}, at::kFloat);
+    entropy = out.take({R}, at::kFloat);
+    lse = out.take({R}, at::kFloat);
+    ids = out.take({R, k}, at::kInt);
+    top = out.take({R, k}, at::kFloat);
   }
   const int rc = mt_token_logprobs(ptr(x), R > 1 ? x.stride(0) : V, ptr<int32_t>(tokens), R, V,
                                    static_cast<int>(k < 1000 ? k : 1000), tokens ? ptr<float>(lp) : nullptr,

@@ -2,7 +2,7 @@
 // alternatives of each row of logits, in one pass over the logits.
 #include <cooperative_groups.h>
 
-#include "mt_common.cuh"
+#include "paged_common.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -38,27 +38,6 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ int key_index(uint64_t key) {
   return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// two fp32 operations in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return d;
 }
 
 // A 16-byte vector of logits: its maximum (NaN skipped where there is another
@@ -122,7 +101,7 @@ struct Sums {
   float2 s, t;
   float M, ref;  // ref: the value M belongs to
   __device__ __forceinline__ void raise(float v) {
-    const float m = rintf(v * kLog2e), d = M - m, f = ex2(d);
+    const float m = rintf(v * kLog2e), d = M - m, f = exp2_approx(d);
     t.x = f * fmaf(d, s.x, t.x);
     t.y = f * fmaf(d, s.y, t.y);
     s.x *= f;
@@ -132,7 +111,7 @@ struct Sums {
   }
   __device__ __forceinline__ void add(float2 x) {
     const float2 z = fma2(x, make_float2(kLog2e, kLog2e), make_float2(-M, -M));
-    const float2 p = make_float2(ex2(z.x), ex2(z.y));
+    const float2 p = make_float2(exp2_approx(z.x), exp2_approx(z.y));
     s = add2(s, p);
     t = fma2(p, z, t);
   }
@@ -390,7 +369,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
 
   // the block's sums, relative to the largest M
   const float mw = warp_max(a.M);
-  float d = a.M - mw, f = ex2(d);
+  float d = a.M - mw, f = exp2_approx(d);
   float s = a.s.x + a.s.y, t = a.t.x + a.t.y;
   t = warp_sum(f * fmaf(d, s, t));
   s = warp_sum(f * s);
@@ -416,7 +395,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
     const float mr = lane < kWarps ? sm.red[0][lane] : -INFINITY;
     const float mb = warp_max(mr);
     d = lane < kWarps ? mr - mb : 0.f;
-    f = lane < kWarps ? ex2(d) : 0.f;
+    f = lane < kWarps ? exp2_approx(d) : 0.f;
     s = lane < kWarps ? sm.red[1][lane] : 0.f;
     t = lane < kWarps ? sm.red[2][lane] : 0.f;
     t = warp_sum(f * fmaf(d, s, t));

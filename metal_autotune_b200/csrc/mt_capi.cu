@@ -127,6 +127,63 @@ int make_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int el
   return MT_OK;
 }
 
+// Encoding a map takes the driver 1.3 us and a call that reads a layout usually
+// reads the same layout again, at other addresses: the last layout encoded by
+// this thread is kept, and a map of it only gets its address set.
+int make_tmaps(CUtensorMap* map0, const void* base0, CUtensorMap* map1, const void* base1, CUtensorMapDataType dt,
+               int elem_bytes, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+               CUtensorMapSwizzle swizzle) {
+  using ReplaceFn = CUresult (*)(CUtensorMap*, void*);
+  static ReplaceFn replace = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapReplaceAddress", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      replace = reinterpret_cast<ReplaceFn>(p);
+  });
+  struct Layout {
+    CUtensorMapDataType dt;
+    CUtensorMapSwizzle swizzle;
+    int elem_bytes, rank;
+    uint64_t dims[5], strides[4];
+    uint32_t box[5];
+  };
+  Layout want;
+  memset(&want, 0, sizeof(want));
+  want.dt = dt;
+  want.swizzle = swizzle;
+  want.elem_bytes = elem_bytes;
+  want.rank = rank;
+  for (int i = 0; i < rank && i < 5; ++i) {
+    want.dims[i] = dims[i];
+    want.box[i] = box[i];
+    if (i + 1 < rank) want.strides[i] = strides[i];
+  }
+  static thread_local Layout last = {};
+  static thread_local CUtensorMap last_map;
+  if (!replace || memcmp(&want, &last, sizeof(want)) != 0) {
+    last.rank = 0;
+    if (int e = make_tmap(&last_map, base0, dt, elem_bytes, rank, dims, strides, box, swizzle)) return e;
+    last = want;
+  }
+  *map0 = last_map;
+  *map1 = last_map;
+  if (!replace) return make_tmap(map1, base1, dt, elem_bytes, rank, dims, strides, box, swizzle);
+  if (!aligned(base0, 16) || !aligned(base1, 16)) {
+    set_error("tensor map: bases %p and %p break the 16-byte rule", base0, base1);
+    return MT_ERR_INVALID_ARGUMENT;
+  }
+  CUresult r = replace(map0, const_cast<void*>(base0));
+  if (r == CUDA_SUCCESS) r = replace(map1, const_cast<void*>(base1));
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapReplaceAddress failed (%d)", (int)r);
+    return MT_ERR_CUDA;
+  }
+  return MT_OK;
+}
+
 int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elem_bytes,
                  uint64_t inner, uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner,
                  uint32_t box_outer, CUtensorMapSwizzle swizzle) {

@@ -18,4 +18,10 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int
 int make_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elem_bytes, int rank,
               const uint64_t* dims, const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle);
 
+// Two maps of one layout at two addresses; encodes only where the layout is not
+// the one this thread encoded last.
+int make_tmaps(CUtensorMap* map0, const void* base0, CUtensorMap* map1, const void* base1, CUtensorMapDataType dt,
+               int elem_bytes, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+               CUtensorMapSwizzle swizzle);
+
 }  // namespace mt

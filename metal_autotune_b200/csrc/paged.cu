@@ -1,7 +1,7 @@
 // Paged serving, per step and per layer: the step's plan (block tables, slots
 // and positions from request lengths) and the q/k prologue that rotates each
 // row at its own position and writes k and v to their slots of the cache.
-#include "mt_common.cuh"
+#include "paged_common.cuh"
 
 namespace mt {
 namespace {
@@ -58,7 +58,7 @@ struct PlanArgs {
   int64_t table_stride, max_pages;
   const int32_t *free_pages, *free_head;
   int64_t n_free;
-  int page_size;
+  FastDiv page;
   int64_t cap;
   int32_t *seq_lens, *query_start, *positions, *token_seq;
   int64_t* slots;
@@ -81,23 +81,27 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   griddep_wait();
   griddep_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int ps = a.page_size;
+  const int ps = a.page.d;
   const int n_free = static_cast<int>(a.n_free);
   int head = a.free_head ? *a.free_head : 0;
   head = head < 0 ? 0 : head > n_free ? n_free : head;
   const int avail = n_free - head;
   const int64_t room = a.max_pages * ps < kPlanMax ? a.max_pages * ps : kPlanMax;
   if (tid < 3) red[tid] = 0;
+  auto pages_of = [&](int len) { return len > 0 ? a.page.div(len - 1) + 1 : 0; };
   int tok_base = 0, page_base = 0, refused = 0, taken = 0;
   for (int64_t r0 = 0; r0 < a.B; r0 += kPlanChunk) {
     const int n = static_cast<int>(a.B - r0 < kPlanChunk ? a.B - r0 : kPlanChunk);
+    const int per = (n + kPlanThreads - 1) / kPlanThreads;  // requests to a thread
+    const int top_bit = 1 << (31 - __clz(n));
     int ctx[kPlanItems], fresh[kPlanItems], need[kPlanItems];
     int own = 0;
 #pragma unroll
     for (int i = 0; i < kPlanItems; ++i) {
-      const int r = tid * kPlanItems + i;
-      ctx[i] = r < n ? max(a.ctx[r0 + r], 0) : 0;
-      fresh[i] = r < n ? max(a.fresh[r0 + r], 0) : 0;
+      const int r = tid * per + i;
+      const bool mine = i < per && r < n;
+      ctx[i] = mine ? max(a.ctx[r0 + r], 0) : 0;
+      fresh[i] = mine ? max(a.fresh[r0 + r], 0) : 0;
       own = sat_add(own, fresh[i]);
     }
     int tok_total, page_total;
@@ -105,20 +109,22 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     own = 0;
 #pragma unroll
     for (int i = 0; i < kPlanItems; ++i) {
+      const int r = tid * per + i;
+      need[i] = -1;
+      if (i >= per || r >= n) continue;
       t = sat_add(t, fresh[i]);
       const int64_t total = static_cast<int64_t>(ctx[i]) + fresh[i];
-      const bool fits = t <= a.cap && total <= room;
-      need[i] = fits ? static_cast<int>((total + ps - 1) / ps) - static_cast<int>((static_cast<int64_t>(ctx[i]) + ps - 1) / ps) : -1;
+      if (t <= a.cap && total <= room) need[i] = pages_of(static_cast<int>(total)) - pages_of(ctx[i]);
       own = sat_add(own, max(need[i], 0));
-      if (tid * kPlanItems + i < n) tok_end[tid * kPlanItems + i] = t;
+      tok_end[r] = t;
     }
     int p = plan_scan(own, page_base, scan, page_total);
 #pragma unroll
     for (int i = 0; i < kPlanItems; ++i) {
-      const int r = tid * kPlanItems + i;
+      const int r = tid * per + i;
       p = sat_add(p, max(need[i], 0));
       const bool ok = need[i] == 0 || (need[i] > 0 && p <= avail);
-      if (r < n) {
+      if (i < per && r < n) {
         page_end[r] = p;
         ctx_of[r] = ok ? ctx[i] : ~ctx[i];
         refused += !ok;
@@ -142,34 +148,42 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
       const int c = ctx_of[lo];
       if (c < 0) continue;
       const int first = lo > 0 ? page_end[lo - 1] : page_base;
-      const int had = static_cast<int>((static_cast<int64_t>(c) + ps - 1) / ps);
+      const int had = pages_of(c);
       a.table[(r0 + lo) * a.table_stride + had + (e - first)] = a.free_pages[head + e];
     }
-    // tokens of this chunk
+    // tokens of this chunk, two of a thread's at a time so that their searches and loads overlap
     const int64_t tok_last = tok_total < a.cap ? tok_total : a.cap;
-    for (int64_t k = tok_base + static_cast<int64_t>(blockIdx.x) * kPlanThreads + tid; k < tok_last;
-         k += static_cast<int64_t>(gridDim.x) * kPlanThreads) {
-      int lo = 0, hi = n - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (tok_end[mid] > k) hi = mid; else lo = mid + 1;
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * kPlanThreads;
+    for (int64_t k0 = tok_base + static_cast<int64_t>(blockIdx.x) * kPlanThreads + tid; k0 < tok_last; k0 += 2 * stride) {
+      int at[2] = {0, 0}, block[2], page[2];
+      int64_t pos[2];
+#pragma unroll 1
+      for (int w = top_bit; w > 0; w >>= 1)  // requests that end at the token or before it
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (at[i] + w <= n && tok_end[at[i] + w - 1] <= k0 + i * stride) at[i] += w;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t k = k0 + i * stride;
+        page[i] = -1;
+        if (k >= tok_last) continue;
+        const int lo = at[i], c0 = ctx_of[lo], c = c0 < 0 ? ~c0 : c0;
+        pos[i] = static_cast<int64_t>(c) + (k - (lo > 0 ? tok_end[lo - 1] : tok_base));
+        if (c0 >= 0) {
+          block[i] = a.page.div(static_cast<int>(pos[i]));  // an admitted request ends below 2^31
+          const int had = pages_of(c), first = lo > 0 ? page_end[lo - 1] : page_base;
+          page[i] = block[i] < had ? a.table[(r0 + lo) * a.table_stride + block[i]]
+                                   : a.free_pages[head + first + (block[i] - had)];
+        }
       }
-      const int c0 = ctx_of[lo];
-      const int c = c0 < 0 ? ~c0 : c0;
-      const int start = lo > 0 ? tok_end[lo - 1] : tok_base;
-      const int64_t pos = static_cast<int64_t>(c) + (k - start);
-      int64_t slot = -1;
-      if (c0 >= 0) {
-        const int block = static_cast<int>(pos / ps);
-        const int had = static_cast<int>((static_cast<int64_t>(c) + ps - 1) / ps);
-        const int first = lo > 0 ? page_end[lo - 1] : page_base;
-        const int page = block < had ? a.table[(r0 + lo) * a.table_stride + block]
-                                     : a.free_pages[head + first + (block - had)];
-        if (page >= 0) slot = static_cast<int64_t>(page) * ps + static_cast<int>(pos - static_cast<int64_t>(block) * ps);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t k = k0 + i * stride;
+        if (k >= tok_last) continue;
+        a.positions[k] = static_cast<int>(pos[i] < kPlanMax ? pos[i] : kPlanMax);
+        a.token_seq[k] = static_cast<int>(r0 + at[i]);
+        a.slots[k] = page[i] >= 0 ? static_cast<int64_t>(page[i]) * ps + (static_cast<int>(pos[i]) - block[i] * ps) : -1;
       }
-      a.positions[k] = static_cast<int>(pos < kPlanMax ? pos : kPlanMax);
-      a.token_seq[k] = static_cast<int>(r0 + lo);
-      a.slots[k] = slot;
     }
     tok_base = tok_total;
     page_base = page_total;
@@ -277,22 +291,6 @@ __device__ __forceinline__ int64_t slot_offset(const AppendArgs& a, int64_t slot
   if (page < a.num_pages) return page * a.page_stride + (slot - page * a.page_size) * a.slot_stride;
   report_status(0x701);
   return -1;
-}
-
-// two fp32 operations in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return d;
 }
 
 // the 16 bytes of a piece of a row as pairs of fp32, and back with one rounding
@@ -622,7 +620,7 @@ int mt_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int64_t B, i
   int sms = 148;
   if (int rc = device_sm_count(&sms)) return rc;
   const PlanArgs a = {ctx_lens, new_lens, B, block_table, table_stride, max_pages, free_pages, free_head, n_free,
-                      (int)page_size, token_cap, seq_lens, query_start, positions, token_seq, slots, counts};
+                      FastDiv::of((int)page_size), token_cap, seq_lens, query_start, positions, token_seq, slots, counts};
   const size_t smem = 3 * sizeof(int) * kPlanChunk;
   if (int rc = ensure_smem(plan_kernel, smem)) return rc;
   const int64_t want = (token_cap + kPlanThreads - 1) / kPlanThreads;
