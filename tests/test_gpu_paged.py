@@ -245,6 +245,21 @@ def test_append_offsets_past_32_bits(cuda):
     assert torch.equal(o[0].view(Hkv, 4, D), v[0][:, None].expand(Hkv, 4, D))
 
 
+def test_attend_offsets_past_32_bits(cuda):
+    """Pages more than 2^31 elements into the cache, by the copy engine and row by row."""
+    D, Hkv, page, pages = 64, 4, 32, 270000  # 2.2e9 elements
+    g = gen(2)
+    kc, vc = (torch.empty(pages, Hkv, page, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    rows = torch.tensor([pages - 1, 3, pages - 2], device="cuda")
+    for c in (kc, vc):
+        c[rows] = torch.randn(3, Hkv, page, D, generator=g, device="cuda").half()
+    q = torch.randn(1, 8, D, generator=g, device="cuda").half()
+    table = rows[None].int()
+    check_attend(q, kc, vc, table, i32([90]), 0.125, "f16")
+    # the same rows as pages of 31 whose last row is never a key: no whole boxes
+    check_attend(q, kc[:, :, :31], vc[:, :, :31], table, i32([93]), 0.125, "f16")
+
+
 # ------------------------------------------------------------------ attention
 def attend_ref(q, kc, vc, table, lens, scale):
     """64-bit result and sum p|v| per output value; keys on pages outside the cache are left out."""
@@ -311,6 +326,10 @@ ATTEND = [
     ([20000, 3, 0, 9000, 1], 5, 1, 128, 16, "f16", "nhd"),
     ([1] * 700, 2, 1, 64, 4, "bf16", "hnd"),               # more requests than CTAs, one key each
     (list(range(0, 1400, 7)), 8, 2, 128, 16, "bf16", "hnd"),
+    ([(37 * i) % 301 for i in range(600)], 32, 8, 128, 16, "bf16", "hnd"),  # many short requests, more than are scanned at once
+    ([(37 * i) % 301 for i in range(600)], 8, 8, 64, 12, "f16", "nhd"),
+    ([400 + (91 * i) % 300 for i in range(300)], 6, 1, 128, 8, "bf16", "nhd"),
+    ([2000, 0, 1, 900, 4097], 48, 4, 128, 32, "f16", "hnd"),  # 12 rows a head
 ]
 
 
