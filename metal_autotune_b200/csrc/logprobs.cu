@@ -2,6 +2,8 @@
 // alternatives of each row of logits, in one pass over the logits.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "paged_common.cuh"
 
 namespace cg = cooperative_groups;
@@ -142,7 +144,8 @@ __device__ __forceinline__ uint64_t take(uint64_t list, uint64_t rising, int lan
 }
 
 struct Slice {  // what a CTA found in its part of a row
-  double m, s, t;  // sum e^(x-m), sum e^(x-m) (x-m); s = 0 where every logit is -inf
+  double m;    // as m ln 2 of a whole m, or the largest logit itself: exact where the sums' rounding would show
+  float s, t;  // sum e^(x-m), sum e^(x-m) (x-m); s = 0 where every logit is -inf
   uint64_t list[kMaxTop];
 };
 
@@ -176,7 +179,7 @@ struct LogprobArgs {
   const void* logits;
   int64_t stride, V;
   const int32_t* tokens;
-  int top_k, split;
+  int top_k, split_bits;  // 2^split_bits CTAs to a row
   float *logprob, *entropy, *lse;
   int32_t* top_ids;
   float* top_lp;
@@ -238,8 +241,8 @@ __device__ __noinline__ void exact_slice(Smem& sm, const Part<DT>& p, int top_k)
       t += sm.red_d[1][w];
     }
     sm.out.m = m;
-    sm.out.s = s;
-    sm.out.t = t;
+    sm.out.s = static_cast<float>(s);
+    sm.out.t = static_cast<float>(t);
   }
   if (top_k == 0) return;
   for (int64_t j0 = 0; j0 < n; j0 += kThreads) {
@@ -403,7 +406,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
     if (lane == 0) {
       sm.out.m = static_cast<double>(mb) * kLn2;
       sm.out.s = s;
-      sm.out.t = t * kLn2;
+      sm.out.t = t * static_cast<float>(kLn2);
       // the largest value alone adds over 1/2, unless it lies below kFloor or the row holds NaN or +inf
       sm.exact = !(s >= 0.25f && s < INFINITY && t == t);
     }
@@ -467,41 +470,44 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const Lo
   griddep_wait();
   griddep_launch();
   const int tid = threadIdx.x, lane = tid & 31;
-  const int64_t row = blockIdx.x / a.split;
-  const int rank = static_cast<int>(blockIdx.x - row * a.split);
+  const int split = 1 << a.split_bits;
+  const int64_t row = blockIdx.x >> a.split_bits;
+  const int rank = blockIdx.x & (split - 1);
   Part<DT> p;
   p.x = static_cast<const T*>(a.logits) + row * a.stride;
   const int off = static_cast<int>((reinterpret_cast<uintptr_t>(p.x) & 15) / sizeof(T));
   p.body = min(static_cast<int64_t>((E - off) % E), a.V);
   const int64_t nvec = (a.V - p.body) / E;
   p.tail0 = p.body + nvec * E;
-  p.v0 = nvec * rank / a.split;
-  p.v1 = nvec * (rank + 1) / a.split;
+  p.v0 = nvec * rank >> a.split_bits;
+  p.v1 = nvec * (rank + 1) >> a.split_bits;
   p.head = rank == 0 ? static_cast<int>(p.body) : 0;
   p.tail = rank == 0 ? static_cast<int>(a.V - p.tail0) : 0;
   if (!one_pass<DT>(sm, p, a.top_k)) exact_slice<DT>(sm, p, a.top_k);
   __syncthreads();
-  double m = sm.out.m, s = sm.out.s, t = sm.out.t;
+  double m = sm.out.m;
+  float s = sm.out.s, t = sm.out.t;
   uint64_t list = tid < 32 ? sm.out.list[lane] : 0;
-  if (a.split > 1) {
+  if (split > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     if (rank == 0) {
       const int warp = tid >> 5;
       if (a.top_k > 0) {  // a list per warp
-        if (warp < a.split) list = cluster.map_shared_rank(&sm.out, warp)->list[lane];
-        list = join_lists(sm, list, a.split);
+        if (warp < split) list = cluster.map_shared_rank(&sm.out, warp)->list[lane];
+        list = join_lists(sm, list, split);
       }
       if (warp == 0) {  // sums, a slice per lane of each eight
         const int c = lane & (kMaxSplit - 1);
-        const Slice* o = cluster.map_shared_rank(&sm.out, c < a.split ? c : 0);
-        const double om = o->m, os = c < a.split ? o->s : 0.0, ot = o->t;
-        m = os == 0 ? -INFINITY : om;  // a slice of -inf alone, or a lane without one
+        const Slice* o = cluster.map_shared_rank(&sm.out, c < split ? c : 0);
+        const double om = o->m;
+        const float os = c < split ? o->s : 0.f, ot = o->t;
+        m = os == 0.f ? -INFINITY : om;  // a slice of -inf alone, or a lane without one
 #pragma unroll
         for (int q = kMaxSplit / 2; q > 0; q >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, q));
-        const double f = exp(om - m);
-        s = os == 0 ? 0.0 : f * os;
-        t = os == 0 ? 0.0 : f * (ot + (om - m) * os);
+        const float d = static_cast<float>(om - m), f = exp2_approx(d * kLog2e);
+        s = os == 0.f ? 0.f : f * os;
+        t = f == 0.f || os == 0.f ? 0.f : f * fmaf(d, os, ot);  // (d may be past the range of floats)
 #pragma unroll
         for (int q = kMaxSplit / 2; q > 0; q >>= 1) {
           s += __shfl_xor_sync(0xffffffffu, s, q);
@@ -513,10 +519,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const Lo
     if (rank != 0) return;
   }
   if (tid >= 32) return;
-  const double ls = s > 0 ? log(s) : NAN, lse = m + ls;  // no distribution: NaN throughout
+  const float ls = s > 0.f ? logf(s) : NAN;  // no distribution: NaN throughout
+  const double lse = m + ls;
   if (lane == 0) {
     if (a.lse) a.lse[row] = static_cast<float>(lse);
-    if (a.entropy) a.entropy[row] = static_cast<float>(ls - t / s);
+    if (a.entropy) a.entropy[row] = ls - t / s;
     if (a.tokens) {
       const int tok = a.tokens[row];
       if (tok >= a.V) report_status(0x801);
@@ -552,12 +559,18 @@ extern "C" int mt_token_logprobs(const void* logits, int64_t row_stride, const i
   MT_CHECK_ARG(aligned(logits, dtype == MT_F32 ? 4 : 2), "mt_token_logprobs: logits not aligned to their type");
   int sms = 148;
   if (int rc = device_sm_count(&sms)) return rc;
-  int split = 1;
-  while (split < kMaxSplit && R * split * 2 <= kCtasPerSm * sms && V / (split * 2) >= 4096) split *= 2;
-  const LogprobArgs a = {logits, row_stride, V, tokens, top_k, split, logprob, entropy, lse, top_ids, top_logprobs};
+  int bits = 0;
+  while ((2 << bits) <= kMaxSplit && (R << (bits + 1)) <= kCtasPerSm * sms && (V >> (bits + 1)) >= 4096) ++bits;
+  const LogprobArgs a = {logits, row_stride, V, tokens, top_k, bits, logprob, entropy, lse, top_ids, top_logprobs};
+  // where there are fewer CTAs than fit, as much shared memory as leaves every SM its share of them: clusters are else
+  // packed onto some of the SMs
+  // (and a little more room for clusters of 8, which do not come out even over the SMs)
+  const int64_t ctas = R << bits, share = ((bits == 3 ? ctas + ctas / 4 : ctas) + sms - 1) / sms;
+  size_t smem = sizeof(Smem);
+  if (share < kCtasPerSm) smem = std::max(smem, static_cast<size_t>(228 * 1024 / share - 1024) / 1024 * 1024);
   auto run = [&](auto kern) -> int {
-    if (int e = ensure_smem(kern, sizeof(Smem))) return e;
-    return launch_cluster(kern, dim3((unsigned)(R * split)), dim3(kThreads), sizeof(Smem), split, (cudaStream_t)stream, a);
+    if (int e = ensure_smem(kern, 227 * 1024)) return e;
+    return launch_cluster(kern, dim3((unsigned)(R << bits)), dim3(kThreads), smem, 1 << bits, (cudaStream_t)stream, a);
   };
   return dtype == MT_BF16  ? run(logprobs_kernel<MT_BF16>)
          : dtype == MT_F16 ? run(logprobs_kernel<MT_F16>)

@@ -12,8 +12,7 @@ namespace {
 // sums of non-negative numbers that saturate at INT32_MAX, so adding in any
 // grouping gives the same result and nothing overflows, whatever the lengths.
 constexpr int kPlanThreads = 512;
-constexpr int kPlanItems = 8;
-constexpr int kPlanChunk = kPlanThreads * kPlanItems;  // requests scanned at a time
+constexpr int kPlanItems = 8;  // requests to a thread at a time; 1 where there are no more than threads
 constexpr int kPlanMax = 0x7fffffff;
 
 __device__ __forceinline__ int sat_add(int a, int b) {
@@ -71,11 +70,15 @@ struct PlanArgs {
 // outputs are then shared out over the grid, each found by a binary search. A
 // token on a new page takes the page from the free list directly, so no CTA
 // reads a table entry that another one writes.
+template <int kItems>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
+  constexpr int kPlanChunk = kPlanThreads * kItems;
+  // a place in eight is left out, so that threads with eight requests each do not meet in a bank
+  auto pad = [](int r) { return r + (r >> 3); };
   extern __shared__ int plan_smem[];
   int* tok_end = plan_smem;                  // inclusive sums of new tokens
-  int* page_end = tok_end + kPlanChunk;      // inclusive sums of new pages
-  int* ctx_of = page_end + kPlanChunk;       // cached tokens; ~cached where the request is refused
+  int* page_end = tok_end + pad(kPlanChunk);  // inclusive sums of new pages
+  int* ctx_of = page_end + pad(kPlanChunk);       // cached tokens; ~cached where the request is refused
   __shared__ PlanScan scan;
   __shared__ int red[3];
   griddep_wait();
@@ -88,50 +91,63 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   const int avail = n_free - head;
   const int64_t room = a.max_pages * ps < kPlanMax ? a.max_pages * ps : kPlanMax;
   if (tid < 3) red[tid] = 0;
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.ctx) | reinterpret_cast<uintptr_t>(a.fresh)) & 15) == 0;
   auto pages_of = [&](int len) { return len > 0 ? a.page.div(len - 1) + 1 : 0; };
   int tok_base = 0, page_base = 0, refused = 0, taken = 0;
   for (int64_t r0 = 0; r0 < a.B; r0 += kPlanChunk) {
     const int n = static_cast<int>(a.B - r0 < kPlanChunk ? a.B - r0 : kPlanChunk);
-    const int per = (n + kPlanThreads - 1) / kPlanThreads;  // requests to a thread
     const int top_bit = 1 << (31 - __clz(n));
-    int ctx[kPlanItems], fresh[kPlanItems], need[kPlanItems];
+    alignas(16) int ctx[kItems], fresh[kItems];
+    int need[kItems];
     int own = 0;
+    if (kItems == 8 && vec && tid * 8 + 8 <= n) {
 #pragma unroll
-    for (int i = 0; i < kPlanItems; ++i) {
-      const int r = tid * per + i;
-      const bool mine = i < per && r < n;
-      ctx[i] = mine ? max(a.ctx[r0 + r], 0) : 0;
-      fresh[i] = mine ? max(a.fresh[r0 + r], 0) : 0;
+      for (int i = 0; i < kItems; i += 4) {
+        *reinterpret_cast<int4*>(ctx + i) = *reinterpret_cast<const int4*>(a.ctx + r0 + tid * 8 + i);
+        *reinterpret_cast<int4*>(fresh + i) = *reinterpret_cast<const int4*>(a.fresh + r0 + tid * 8 + i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int r = tid * kItems + i;
+        ctx[i] = r < n ? a.ctx[r0 + r] : 0;
+        fresh[i] = r < n ? a.fresh[r0 + r] : 0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      ctx[i] = max(ctx[i], 0);
+      fresh[i] = max(fresh[i], 0);
       own = sat_add(own, fresh[i]);
     }
     int tok_total, page_total;
     int t = plan_scan(own, tok_base, scan, tok_total);
     own = 0;
 #pragma unroll
-    for (int i = 0; i < kPlanItems; ++i) {
-      const int r = tid * per + i;
+    for (int i = 0; i < kItems; ++i) {
+      const int r = tid * kItems + i;
       need[i] = -1;
-      if (i >= per || r >= n) continue;
+      if (r >= n) continue;
       t = sat_add(t, fresh[i]);
       const int64_t total = static_cast<int64_t>(ctx[i]) + fresh[i];
       if (t <= a.cap && total <= room) need[i] = pages_of(static_cast<int>(total)) - pages_of(ctx[i]);
       own = sat_add(own, max(need[i], 0));
-      tok_end[r] = t;
+      tok_end[pad(r)] = t;
     }
     int p = plan_scan(own, page_base, scan, page_total);
 #pragma unroll
-    for (int i = 0; i < kPlanItems; ++i) {
-      const int r = tid * per + i;
+    for (int i = 0; i < kItems; ++i) {
+      const int r = tid * kItems + i;
       p = sat_add(p, max(need[i], 0));
       const bool ok = need[i] == 0 || (need[i] > 0 && p <= avail);
-      if (i < per && r < n) {
-        page_end[r] = p;
-        ctx_of[r] = ok ? ctx[i] : ~ctx[i];
+      if (r < n) {
+        page_end[pad(r)] = p;
+        ctx_of[pad(r)] = ok ? ctx[i] : ~ctx[i];
         refused += !ok;
         if (ok && need[i] > 0) taken = p;
         if (warp % gridDim.x == blockIdx.x) {
           a.seq_lens[r0 + r] = ok ? ctx[i] + fresh[i] : ctx[i];
-          a.query_start[r0 + r + 1] = tok_end[r];
+          a.query_start[r0 + r + 1] = tok_end[pad(r)];
         }
       }
     }
@@ -143,11 +159,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
       int lo = 0, hi = n - 1;  // first request with page_end > e
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (page_end[mid] > e) hi = mid; else lo = mid + 1;
+        if (page_end[pad(mid)] > e) hi = mid; else lo = mid + 1;
       }
-      const int c = ctx_of[lo];
+      const int c = ctx_of[pad(lo)];
       if (c < 0) continue;
-      const int first = lo > 0 ? page_end[lo - 1] : page_base;
+      const int first = lo > 0 ? page_end[pad(lo - 1)] : page_base;
       const int had = pages_of(c);
       a.table[(r0 + lo) * a.table_stride + had + (e - first)] = a.free_pages[head + e];
     }
@@ -161,17 +177,17 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
       for (int w = top_bit; w > 0; w >>= 1)  // requests that end at the token or before it
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          if (at[i] + w <= n && tok_end[at[i] + w - 1] <= k0 + i * stride) at[i] += w;
+          if (at[i] + w <= n && tok_end[pad(at[i] + w - 1)] <= k0 + i * stride) at[i] += w;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int64_t k = k0 + i * stride;
         page[i] = -1;
         if (k >= tok_last) continue;
-        const int lo = at[i], c0 = ctx_of[lo], c = c0 < 0 ? ~c0 : c0;
-        pos[i] = static_cast<int64_t>(c) + (k - (lo > 0 ? tok_end[lo - 1] : tok_base));
+        const int lo = at[i], c0 = ctx_of[pad(lo)], c = c0 < 0 ? ~c0 : c0;
+        pos[i] = static_cast<int64_t>(c) + (k - (lo > 0 ? tok_end[pad(lo - 1)] : tok_base));
         if (c0 >= 0) {
           block[i] = a.page.div(static_cast<int>(pos[i]));  // an admitted request ends below 2^31
-          const int had = pages_of(c), first = lo > 0 ? page_end[lo - 1] : page_base;
+          const int had = pages_of(c), first = lo > 0 ? page_end[pad(lo - 1)] : page_base;
           page[i] = block[i] < had ? a.table[(r0 + lo) * a.table_stride + block[i]]
                                    : a.free_pages[head + first + (block[i] - had)];
         }
@@ -621,11 +637,14 @@ int mt_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int64_t B, i
   if (int rc = device_sm_count(&sms)) return rc;
   const PlanArgs a = {ctx_lens, new_lens, B, block_table, table_stride, max_pages, free_pages, free_head, n_free,
                       FastDiv::of((int)page_size), token_cap, seq_lens, query_start, positions, token_seq, slots, counts};
-  const size_t smem = 3 * sizeof(int) * kPlanChunk;
-  if (int rc = ensure_smem(plan_kernel, smem)) return rc;
   const int64_t want = (token_cap + kPlanThreads - 1) / kPlanThreads;
   const int64_t grid = want < 1 ? 1 : want < sms ? want : sms;
-  return launch(plan_kernel, dim3((unsigned)grid), dim3(kPlanThreads), smem, (cudaStream_t)stream, a);
+  auto run = [&](auto kern, int items) -> int {
+    const size_t smem = 3 * sizeof(int) * (kPlanThreads * items + kPlanThreads * items / 8);
+    if (int rc = ensure_smem(kern, smem)) return rc;
+    return launch(kern, dim3((unsigned)grid), dim3(kPlanThreads), smem, (cudaStream_t)stream, a);
+  };
+  return B <= kPlanThreads ? run(plan_kernel<1>, 1) : run(plan_kernel<kPlanItems>, kPlanItems);
 }
 
 int mt_rope_paged_append(const void* q, const void* k, const void* v, int64_t q_st, int64_t q_sh, int64_t k_st,
