@@ -32,7 +32,6 @@ struct PagedParams {
 constexpr int kWarps = 4;                   // that compute; as many fetch, one for each
 constexpr int kThreads = kWarps * 32;       // that compute
 constexpr int kCtaThreads = 2 * kThreads;
-constexpr int kKeys = 16;      // keys of one warp's step
 // What a unit's beginning and end count as, in steps, when the work is cut: 64 requests of 64..8192 keys (32/8 heads of
 // 128, bf16) 85.6 us without, 80.3 with 1, 78.2 with 2; 256 of 1..512 40.8, 29.9, 28.5.
 constexpr int kUnitCost = 2;
@@ -48,10 +47,11 @@ constexpr int kMaxCtas = 444;  // bounds the workspace; 3 CTAs on each of 148 SM
 constexpr size_t kWsPagedCtl = kWsQmmDone;
 static_assert(kWsPagedCtl + 4 * kMaxCtas * kWarps <= kWsCtlBytes, "the counters are control words");
 
-// Byte offset of a 16-byte chunk of a staged row: 64-element halves of the 16
+// Byte offset of a 16-byte chunk of a staged row: 64-element halves of the KEYS
 // rows one after another, each as the copy engine's 128-byte swizzle lays it out.
+template <int KEYS>
 __device__ __forceinline__ uint32_t swz(int row, int chunk) {
-  return static_cast<uint32_t>(((chunk >> 3) << 11) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+  return static_cast<uint32_t>((chunk >> 3) * (KEYS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
 // a / b for non-negative numbers, by 32-bit division where they fit
@@ -61,8 +61,8 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 }
 
 // Where a worker's copies stand in the flattened steps of (request, kv head x
-// row block): 16 keys of a warp that works by itself, 64 of a CTA whose warps
-// take 16 each. A unit of nt steps takes nt + kUnitCost places in the order:
+// row block): KEYS keys of a warp that works by itself, four times as many of a
+// CTA whose warps take KEYS each. A unit of nt steps takes nt + kUnitCost places in the order:
 // its beginning and end cost as much as that many steps.
 //
 // The table's entries come in by windows of 32, a lane each, the next window
@@ -98,7 +98,8 @@ struct Loader {
     }
     ahead = ahead_b == b && ahead_base == base ? win : entry(p, ahead_b, ahead_base, len_, lane);
   }
-  // the page of this lane's key (lane modulo 16) of the step at key0
+  // the page of this lane's key (lane modulo KEYS) of the step at key0
+  template <int KEYS>
   __device__ __forceinline__ int page_of(const PagedParams& p, int key0, int heads, int lane) {
     const int i0 = p.page.div(min(key0, len - 1));
     if (ahead_b == b && ahead_base == (i0 & ~31) && base != ahead_base) {
@@ -110,7 +111,7 @@ struct Loader {
       win = entry(p, b, base, len, lane);
       look_ahead(p, heads, lane);
     }
-    const int key = key0 + (lane & 15);
+    const int key = key0 + (lane & (KEYS - 1));
     const int i = p.page.div(min(key, len - 1)) - base;
     int page = __shfl_sync(0xffffffffu, win, i & 31);
     if (__any_sync(0xffffffffu, i >= 32)) {  // (only then wait for the next window)
@@ -150,52 +151,57 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-// The step's 16 rows of K and V into stage memory, completing on `bar`. Rows
+// The step's KEYS rows of K and V into stage memory, completing on `bar`. Rows
 // without a key (past the length, or on a page id outside the cache) stay out
-// of the mask. BOX: the copy engine fetches boxes of 8 or 16 rows that lie in
-// one page (the page size is a multiple of that), 128 bytes of each row.
+// of the mask. BOX: the copy engine fetches boxes of 8, 16 or 32 rows that lie
+// in one page (the page size is a multiple of that), 128 bytes of each row.
 // Otherwise 16-byte asynchronous copies, each row from where its page is.
-template <int D, bool BOX>
+template <int D, int KEYS, bool BOX>
 __device__ __forceinline__ void load_step(const PagedParams& p, const CUtensorMap* kmap, const CUtensorMap* vmap,
                                           const Loader& c, int page, int key0, int lane, uint8_t* stage,
                                           uint32_t* mask, uint64_t* bar) {
-  const int key = key0 + (lane & 15);
+  const int key = key0 + (lane & (KEYS - 1));
   const bool there = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.num_pages);
   if (key < c.len && !there) report_status(0x702);
-  const uint32_t m = __ballot_sync(0xffffffffu, key < c.len && there) & 0xffffu;
+  const uint32_t m = __ballot_sync(0xffffffffu, key < c.len && there) & (KEYS == 32 ? ~0u : 0xffffu);
   if (lane == 0) *mask = m;
   if constexpr (BOX) {
-    const int rows = p.box_rows, page8 = __shfl_sync(0xffffffffu, page, 8);
+    int pages[KEYS / 8];
+    uint32_t boxes = 0;
+#pragma unroll
+    for (int g = 0; g < KEYS / 8; ++g) {
+      pages[g] = __shfl_sync(0xffffffffu, page, 8 * g);
+      boxes += (8 * g & (p.box_rows - 1)) == 0 && (m >> (8 * g)) & 1;
+    }
     if (lane == 0) {
-      const bool two = rows == 8 && (m >> 8) & 1;
-      mbar_arrive_expect_tx(bar, ((m & 1) + two) * rows * D * 4);
-      auto fetch = [&](int first, int at_page) {
-        const int slot = key0 + first - p.page.div(key0 + first) * p.page.d;
+      mbar_arrive_expect_tx(bar, boxes * p.box_rows * D * 4);
+#pragma unroll
+      for (int g = 0; g < KEYS / 8; ++g) {
+        if ((8 * g & (p.box_rows - 1)) != 0 || !((m >> (8 * g)) & 1)) continue;
+        const int first = key0 + 8 * g, slot = first - p.page.div(first) * p.page.d;
 #pragma unroll
         for (int half = 0; half < D / 64; ++half) {
-          uint8_t* dst = stage + half * 2048 + first * 128;
-          tma_load_4d(dst, kmap, bar, half * 64, slot, c.hk, at_page);
-          tma_load_4d(dst + kKeys * D * 2, vmap, bar, half * 64, slot, c.hk, at_page);
+          uint8_t* dst = stage + half * KEYS * 128 + g * 1024;
+          tma_load_4d(dst, kmap, bar, half * 64, slot, c.hk, pages[g]);
+          tma_load_4d(dst + KEYS * D * 2, vmap, bar, half * 64, slot, c.hk, pages[g]);
         }
-      };
-      if (m & 1) fetch(0, page);
-      if (two) fetch(8, page8);
+      }
     }
   } else {
     constexpr int CPR = D / 8;     // 16-byte chunks per row
     constexpr int RPI = 32 / CPR;  // rows per instruction
     const int chunk = lane % CPR;
     int64_t off = 0;
-    if ((m >> (lane & 15)) & 1)
+    if ((m >> (lane & (KEYS - 1))) & 1)
       off = page * p.page_stride + (key - p.page.div(key) * p.page.d) * p.slot_stride + c.hk * p.head_stride;
 #pragma unroll
-    for (int i = 0; i < kKeys / RPI; ++i) {
+    for (int i = 0; i < KEYS / RPI; ++i) {
       const int row = i * RPI + lane / CPR;
       const int64_t src = __shfl_sync(0xffffffffu, off, row) + chunk * 8;
       if ((m >> row) & 1) {
-        const uint32_t at = swz(row, chunk);
+        const uint32_t at = swz<KEYS>(row, chunk);
         cp_async16(stage + at, static_cast<const uint16_t*>(p.kc) + src, true);
-        cp_async16(stage + kKeys * D * 2 + at, static_cast<const uint16_t*>(p.vc) + src, true);
+        cp_async16(stage + KEYS * D * 2 + at, static_cast<const uint16_t*>(p.vc) + src, true);
       }
     }
     // this lane's arrival when its copies have landed, and one that the mask's store comes before
@@ -211,15 +217,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   return d;
 }
 
-template <int D, int R, int kStages>
+template <int D, int R, int KEYS, int kStages>
 struct PagedSmem {
-  static constexpr int kStageBytes = 2 * kKeys * D * 2;
+  static constexpr int kStageBytes = 2 * KEYS * D * 2;
   static constexpr int kOStride = D + 4;
   alignas(1024) uint8_t stage[kWarps][kStages][kStageBytes];
   uint64_t full[kWarps][kStages], empty[kWarps][kStages];
   float m[kWarps][R], l[kWarps][R];
   uint32_t mask[kWarps][kStages];
-  int sum16[2 * kWarps], sum64[2 * kWarps];
+  int sum_solo[2 * kWarps], sum_group[2 * kWarps];
   int longest[2 * kWarps];
   int64_t at_step[kWarps];
   int at_b[kWarps];
@@ -302,26 +308,29 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, int64_t c0, int
 // per worker, whatever the lengths are; a run starts and ends anywhere inside a
 // request. A worker is a warp, where runs are long enough and no request spans
 // many of them: then nothing in the loop or at a request's end waits for
-// another warp. Else it is a CTA whose 4 warps take 16 of every 64 keys and
-// join through shared memory at the request's end. Where a request's keys span
+// another warp. Else it is a CTA whose 4 warps take a quarter each of a step's
+// keys and join through shared memory at the request's end. Where a request's keys span
 // several workers, each leaves its part (maximum, sum, unnormalised output) in
 // the workspace, and the one that arrives last joins them.
 //
 // A warp that computes is fed by one that fetches, through a ring of stages:
 // finding the next keys' page and issuing their copies takes about as long as
-// computing on 16 keys does. The tensor instructions take the keys as their 16
+// computing on them does. The tensor instructions take 16 keys as their
 // rows and the query rows of a kv head as their 8 columns: S^T = K Q^T, then
 // O^T += V^T P^T, so up to 8 query heads of a kv head fill them without
 // padding, and an accumulator takes D/2 registers.
-template <int DT, int D, int R, int kStages, bool BOX, int kPerSm>
+template <int DT, int D, int R, int KEYS, int kStages, bool BOX, int kPerSm>
 __global__ void __launch_bounds__(kCtaThreads, kPerSm)
     paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using T = typename Elem<DT>::T;
   constexpr int KS = D / 16;  // mma steps over the head
   constexpr int NB = R / 8;   // blocks of 8 query rows
+  constexpr int NK = KEYS / 16;  // blocks of 16 keys
+  constexpr int kGroup = kWarps * KEYS;
+  constexpr uint32_t kAll = KEYS == 32 ? ~0u : 0xffffu;
   constexpr int kPart = R * (D + 2);
   extern __shared__ uint8_t smem_raw[];
-  using Smem = PagedSmem<D, R, kStages>;
+  using Smem = PagedSmem<D, R, KEYS, kStages>;
   uint8_t* smem = smem_raw + (1024 - (smem_addr(smem_raw) & 1023)) % 1024;
   Smem& sm = *reinterpret_cast<Smem*>(smem);
   const int rmax = min(R, p.G);
@@ -346,27 +355,27 @@ __global__ void __launch_bounds__(kCtaThreads, kPerSm)
   griddep_wait();
   griddep_launch();
 
-  // all places, by 16 and by 64 keys, and the longest request (the host bounds their sums below 2^31)
+  // all places, of a warp's steps and of a CTA's, and the longest request (the host bounds their sums below 2^31)
   auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.max_len); };
   auto places = [](int len, int keys) { return len > 0 ? (len + keys - 1) / keys + kUnitCost : 0; };
   const int my_len = tid < p.B ? len_of(tid) : 0;
   bool empty = false;  // of the empty requests, those with b = CTA modulo the grid are this CTA's
   {
     empty = tid < p.B && my_len == 0 && tid % gridDim.x == blockIdx.x;
-    int n16 = places(my_len, 16), n64 = places(my_len, 64), longest = my_len;
+    int n_solo = places(my_len, KEYS), n_group = places(my_len, kGroup), longest = my_len;
     for (int b = tid + kCtaThreads; b < p.B; b += kCtaThreads) {
       const int len = len_of(b);
       empty = empty || (len == 0 && b % gridDim.x == blockIdx.x);
-      n16 += places(len, 16);
-      n64 += places(len, 64);
+      n_solo += places(len, KEYS);
+      n_group += places(len, kGroup);
       longest = max(longest, len);
     }
-    n16 = __reduce_add_sync(0xffffffffu, n16);
-    n64 = __reduce_add_sync(0xffffffffu, n64);
+    n_solo = __reduce_add_sync(0xffffffffu, n_solo);
+    n_group = __reduce_add_sync(0xffffffffu, n_group);
     longest = __reduce_max_sync(0xffffffffu, longest);
     if (lane == 0) {
-      sm.sum16[cta_warp] = n16;
-      sm.sum64[cta_warp] = n64;
+      sm.sum_solo[cta_warp] = n_solo;
+      sm.sum_group[cta_warp] = n_group;
       sm.longest[cta_warp] = longest;
     }
   }
@@ -375,23 +384,23 @@ __global__ void __launch_bounds__(kCtaThreads, kPerSm)
       if (len_of(b) == 0)
         for (int i = tid; i < p.Hkv * p.G * D; i += kCtaThreads)
           static_cast<T*>(p.o)[b * p.o_sb + (i / D) * p.o_sh + i % D] = Elem<DT>::from_f(0.f);
-  int n16 = 0, n64 = 0, longest = 0;
+  int n_solo = 0, n_group = 0, longest = 0;
 #pragma unroll
   for (int w = 0; w < 2 * kWarps; ++w) {
-    n16 += sm.sum16[w];
-    n64 += sm.sum64[w];
+    n_solo += sm.sum_solo[w];
+    n_group += sm.sum_group[w];
     longest = max(longest, sm.longest[w]);
   }
   // Which worker: a warp where requests are short (their ends then cost more than the splits) and no request spans
   // many of them.
-  const int64_t solo_quota = quotient(static_cast<int64_t>(n16) * heads + gridDim.x * kWarps - 1, gridDim.x * kWarps);
-  const bool solo = solo_quota >= kSoloRun && n16 / kSoloMean < p.B && (longest + 15) >> 4 <= 24 * solo_quota;
-  const int keys = solo ? 16 : 64, first = solo ? 0 : warp * kKeys;
-  const int64_t total = static_cast<int64_t>(solo ? n16 : n64) * heads;
+  const int64_t solo_quota = quotient(static_cast<int64_t>(n_solo) * heads + gridDim.x * kWarps - 1, gridDim.x * kWarps);
+  const bool solo = solo_quota >= kSoloRun && n_solo / (kSoloMean * 16 / KEYS) < p.B && longest / KEYS < 24 * solo_quota;
+  const int keys = solo ? KEYS : kGroup, first = solo ? 0 : warp * KEYS;
+  const int64_t total = static_cast<int64_t>(solo ? n_solo : n_group) * heads;
   // a CTA's run is no shorter than a short request, or a few steps of a long one: a split costs about four steps
   const int64_t quota =
       solo ? solo_quota
-           : max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<int64_t>(min(places(longest, 64), kLeastRun)));
+           : max(quotient(total + gridDim.x - 1, gridDim.x), static_cast<int64_t>(min(places(longest, kGroup), kLeastRun)));
   const int64_t worker = solo ? static_cast<int64_t>(blockIdx.x) * kWarps + warp : blockIdx.x;
   const int64_t lo = worker * quota, hi = min(lo + quota, total);
   if (blockIdx.x * quota * (solo ? kWarps : 1) >= total) return;
@@ -407,7 +416,7 @@ __global__ void __launch_bounds__(kCtaThreads, kPerSm)
         const int u = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += u;
       }
-      int* sums = solo ? sm.sum16 : sm.sum64;
+      int* sums = solo ? sm.sum_solo : sm.sum_group;
       if (p.B > kCtaThreads) {  // (one chunk: its warps' sums are there already)
         __syncthreads();
         if (lane == 31) sums[cta_warp] = inc;
@@ -461,9 +470,9 @@ __global__ void __launch_bounds__(kCtaThreads, kPerSm)
     int64_t step = 0;
     while (ld.left > 0) {
       const int key0 = ld.t * keys + first;
-      const int page = ld.page_of(p, key0, heads, lane);
+      const int page = ld.page_of<KEYS>(p, key0, heads, lane);
       if (step >= kStages && !mbar_wait_warp(&sm.empty[warp][at], phase ^ 1, &sm.abort, 0x704)) return;  // reported
-      load_step<D, BOX>(p, &kmap, &vmap, ld, page, key0, lane, stages + at * Smem::kStageBytes, &sm.mask[warp][at],
+      load_step<D, KEYS, BOX>(p, &kmap, &vmap, ld, page, key0, lane, stages + at * Smem::kStageBytes, &sm.mask[warp][at],
                         &sm.full[warp][at]);
       if (ld.advance(p, heads, keys)) {  // another request: its first window has come in, or has not
         const bool come = ld.ahead_b == ld.b && ld.ahead_base == 0;
@@ -550,41 +559,54 @@ __global__ void __launch_bounds__(kCtaThreads, kPerSm)
       dead = __any_sync(0xffffffffu, dead);  // reported; nothing more is computed
       const uint32_t mask = dead ? 0u : sm.mask[warp][at];
       uint8_t* stage = stages + at * Smem::kStageBytes;
-      const uint32_t kb = smem_addr(stage), vb = kb + kKeys * D * 2;
+      const uint32_t kaddr = smem_addr(stage), vaddr = kaddr + KEYS * D * 2;
       if (mask != 0) {
-        if (mask != 0xffffu) {  // rows of V without a key are zeros, not what the page or the stage holds there
-          for (int i = lane; i < kKeys * (D / 8); i += 32) {
+        if (mask != kAll) {  // rows of V without a key are zeros, not what the page or the stage holds there
+          for (int i = lane; i < KEYS * (D / 8); i += 32) {
             const int row = i / (D / 8);
             if (!((mask >> row) & 1))
-              *reinterpret_cast<uint4*>(stage + kKeys * D * 2 + swz(row, i % (D / 8))) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(stage + KEYS * D * 2 + swz<KEYS>(row, i % (D / 8))) = make_uint4(0, 0, 0, 0);
           }
           if (BOX) fence_proxy_async_shared();
           __syncwarp();
         }
-        float s[NB][2][4];  // two chains over the head, added at the end
+        constexpr int CH = NK == 1 ? 2 : 1;  // chains over the head for a block of keys, added at the end
+        float s[NK][NB][CH][4];
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+        for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[j][0][i] = s[j][1][i] = 0.f;
+          for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          uint32_t a[4];
-          ldsm_x4(kb + swz(lane & 15, 2 * k + (lane >> 4)), a[0], a[1], a[2], a[3]);
+            for (int c = 0; c < CH; ++c)
 #pragma unroll
-          for (int j = 0; j < NB; ++j) mma16816<DT>(s[j][k & 1], a, qf[k][j], qf[k][NB + j]);
-        }
-        uint32_t pb[NB][2];
+              for (int i = 0; i < 4; ++i) s[kb][j][c][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int kb = 0; kb < NK; ++kb) {
+            uint32_t a[4];
+            ldsm_x4(kaddr + swz<KEYS>(kb * 16 + (lane & 15), 2 * k + (lane >> 4)), a[0], a[1], a[2], a[3]);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) mma16816<DT>(s[kb][j][k % CH], a, qf[k][j], qf[k][NB + j]);
+          }
+        uint32_t pb[NK][NB][2];
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-          // key lane / 4 (+ 8 in x[2], x[3]) and rows 2 (lane % 4), + 1
-          float x[4];
+          // key 16 kb + lane / 4 (+ 8 in x[2], x[3]) and rows 2 (lane % 4), + 1
+          float x[NK][4];
+          float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = (s[j][0][i] + s[j][1][i]) * p.scale_log2;
-          if (mask != 0xffffu) {
-            if (!((mask >> (lane >> 2)) & 1)) x[0] = x[1] = -INFINITY;
-            if (!((mask >> ((lane >> 2) + 8)) & 1)) x[2] = x[3] = -INFINITY;
+          for (int kb = 0; kb < NK; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              x[kb][i] = (CH == 2 ? s[kb][j][0][i] + s[kb][j][CH - 1][i] : s[kb][j][0][i]) * p.scale_log2;
+            if (mask != kAll) {
+              if (!((mask >> (kb * 16 + (lane >> 2))) & 1)) x[kb][0] = x[kb][1] = -INFINITY;
+              if (!((mask >> (kb * 16 + (lane >> 2) + 8)) & 1)) x[kb][2] = x[kb][3] = -INFINITY;
+            }
+            m0 = fmaxf(m0, fmaxf(x[kb][0], x[kb][2]));
+            m1 = fmaxf(m1, fmaxf(x[kb][1], x[kb][3]));
           }
-          float m0 = fmaxf(x[0], x[2]), m1 = fmaxf(x[1], x[3]);
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
@@ -607,21 +629,27 @@ __global__ void __launch_bounds__(kCtaThreads, kPerSm)
             }
           }
           const float r0 = mx[j][0] == -INFINITY ? 0.f : mx[j][0], r1 = mx[j][1] == -INFINITY ? 0.f : mx[j][1];
-          const float e0 = exp2_approx(x[0] - r0), e1 = exp2_approx(x[1] - r1);
-          const float e2 = exp2_approx(x[2] - r0), e3 = exp2_approx(x[3] - r1);
-          sum[j][0] += e0 + e2;
-          sum[j][1] += e1 + e3;
-          // the probabilities in 16 bits, as the product with V takes them
-          pb[j][0] = transpose8(pack2<DT>(e0, e1));
-          pb[j][1] = transpose8(pack2<DT>(e2, e3));
+#pragma unroll
+          for (int kb = 0; kb < NK; ++kb) {
+            const float e0 = exp2_approx(x[kb][0] - r0), e1 = exp2_approx(x[kb][1] - r1);
+            const float e2 = exp2_approx(x[kb][2] - r0), e3 = exp2_approx(x[kb][3] - r1);
+            sum[j][0] += e0 + e2;
+            sum[j][1] += e1 + e3;
+            // the probabilities in 16 bits, as the product with V takes them
+            pb[kb][j][0] = transpose8(pack2<DT>(e0, e1));
+            pb[kb][j][1] = transpose8(pack2<DT>(e2, e3));
+          }
         }
 #pragma unroll
-        for (int n = 0; n < KS; ++n) {
-          uint32_t a[4];
-          ldsm_x4_t(vb + swz((lane & 7) + ((lane >> 4) << 3), 2 * n + ((lane >> 3) & 1)), a[0], a[1], a[2], a[3]);
+        for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-          for (int j = 0; j < NB; ++j) mma16816<DT>(acc[n][j], a, pb[j][0], pb[j][1]);
-        }
+          for (int n = 0; n < KS; ++n) {
+            uint32_t a[4];
+            ldsm_x4_t(vaddr + swz<KEYS>(kb * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * n + ((lane >> 3) & 1)), a[0], a[1],
+                      a[2], a[3]);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) mma16816<DT>(acc[n][j], a, pb[kb][j][0], pb[kb][j][1]);
+          }
       }
       __syncwarp();
       if (dead) continue;  // the stage stays taken: the warp that fetches gives up too
@@ -809,7 +837,7 @@ int mt_paged_sdpa_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* 
   // the copy engine where pages hold whole boxes and its strides can express the cache
   const int64_t bytes[3] = {slot_stride * 2, head_stride * 2, page_stride * 2};
   const int64_t extent[3] = {page_size, Hkv, num_pages};
-  p.box_rows = page_size % 16 == 0 ? 16 : 8;
+  p.box_rows = D == 64 && page_size % 32 == 0 ? 32 : page_size % 16 == 0 ? 16 : 8;
   bool box = page_size % 8 == 0 && num_pages > 0;
   uint64_t dims[4] = {(uint64_t)D}, strides[3];
   for (int i = 0; i < 3; ++i) {
@@ -835,16 +863,19 @@ int mt_paged_sdpa_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* 
   // by head size and query rows: ring stages and CTAs to an SM that its shared memory holds beside the rows to join
   auto pick = [&](auto type, auto dim) -> int {
     constexpr int DT = decltype(type)::value, D_ = decltype(dim)::value;
-    auto with = [&](auto r, auto stages, auto per_sm) -> int {
-      constexpr int R_ = decltype(r)::value, S_ = decltype(stages)::value, N_ = decltype(per_sm)::value;
-      const size_t smem = PagedSmem<D_, R_, S_>::bytes(rows);
-      return box ? run(paged_kernel<DT, D_, R_, S_, true, N_>, smem, N_) : run(paged_kernel<DT, D_, R_, S_, false, N_>, smem, N_);
+    auto with = [&](auto r, auto keys, auto stages, auto per_sm) -> int {
+      constexpr int R_ = decltype(r)::value, K_ = decltype(keys)::value, S_ = decltype(stages)::value,
+                    N_ = decltype(per_sm)::value;
+      const size_t smem = PagedSmem<D_, R_, K_, S_>::bytes(rows);
+      return box ? run(paged_kernel<DT, D_, R_, K_, S_, true, N_>, smem, N_)
+                 : run(paged_kernel<DT, D_, R_, K_, S_, false, N_>, smem, N_);
     };
-    if constexpr (D_ == 64) return R == 8 ? with(Int<8>(), Int<3>(), Int<3>()) : with(Int<16>(), Int<3>(), Int<2>());
+    if constexpr (D_ == 64)
+      return R == 16 ? with(Int<16>(), Int<32>(), Int<2>(), Int<2>()) : with(Int<8>(), Int<32>(), Int<3>(), Int<2>());
     else
-      return R == 16  ? with(Int<16>(), Int<4>(), Int<1>())
-             : G <= 4 ? with(Int<8>(), Int<3>(), Int<2>())
-                      : with(Int<8>(), Int<2>(), Int<2>());
+      return R == 16  ? with(Int<16>(), Int<16>(), Int<4>(), Int<1>())
+             : G <= 4 ? with(Int<8>(), Int<16>(), Int<3>(), Int<2>())
+                      : with(Int<8>(), Int<16>(), Int<2>(), Int<2>());
   };
   if (dtype == MT_BF16) return D == 128 ? pick(Int<MT_BF16>(), Int<128>()) : pick(Int<MT_BF16>(), Int<64>());
   return D == 128 ? pick(Int<MT_F16>(), Int<128>()) : pick(Int<MT_F16>(), Int<64>());
