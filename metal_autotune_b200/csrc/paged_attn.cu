@@ -32,16 +32,17 @@ struct PagedParams {
 constexpr int kWarps = 4;                   // that compute; as many fetch, one for each
 constexpr int kThreads = kWarps * 32;       // that compute
 constexpr int kCtaThreads = 2 * kThreads;
-// What a unit's beginning and end count as, in steps, when the work is cut: 64 requests of 64..8192 keys (32/8 heads of
-// 128, bf16) 85.6 us without, 80.3 with 1, 78.2 with 2; 256 of 1..512 40.8, 29.9, 28.5.
-constexpr int kUnitCost = 2;
+// What a unit's beginning and end count as, in steps, when the work is cut (32/8 heads of 128, bf16): 64 requests of
+// 64..8192 keys 85.6 us without, 80.3 with 1, 78.4 with 2 or 3; 256 of 1..512 40.8, 29.9, 28.4, 27.7; 37 of 0..1500
+// with 20 heads of 64 17.8 with 2, 15.1 with 3 (and the next rule).
+constexpr int kUnitCost = 3;
 // The least run of a CTA, in places, where requests are that long: one request of 129 keys 6.1 us (a CTA to a head, no
-// parts to join), 7.1 cut at every step; four of 4096 19.9 either way.
+// parts to join), 7.1 cut at every step; four of 4096 the same either way.
 constexpr int kLeastRun = 6;
-// Warps work by themselves where a request has fewer places than this on average, and runs are at least so long:
-// 256 requests of 1..512 keys 28.5 us, 34.2 by CTAs; 32 of 1024 33.6, 29.6 by CTAs.
-constexpr int kSoloMean = 16, kSoloRun = 8;
-constexpr int kMaxCtas = 444;  // bounds the workspace; 3 CTAs on each of 148 SMs
+// Warps work by themselves where a request has fewer places than this on average (of 16 keys), and runs are at least so
+// long: 256 requests of 1..512 keys 28.5 us, 34.2 by CTAs; 32 of 1024 33.6, 29.6 by CTAs.
+constexpr int kSoloMean = 24, kSoloRun = 4;
+constexpr int kMaxCtas = 296;  // bounds the workspace; 2 CTAs on each of 148 SMs
 // arrival counters, one per warp of the grid, in the workspace's control words (the quantised matmul's: both leave
 // them zero, and the workspace is used by one kernel at a time)
 constexpr size_t kWsPagedCtl = kWsQmmDone;
