@@ -278,6 +278,12 @@ __device__ __noinline__ void exact_slice(Smem& sm, const Part<DT>& p, int top_k)
 // lower index), so constant or masked stretches stay within the buffer too.
 // Which thread stores a candidate where does not matter: keys are unique and
 // the sort is by key.
+//
+// Memory bounds it for many rows: 2048 x 151936 bf16 with 20 alternatives in
+// 121 us = 5.1 TB/s, 78% of the copy rate (without alternatives 108.6 us, 87%;
+// 223 us when the bound came from the row's beginning and candidates left the
+// loop one by one). The loop runs at the copy rate; what follows it, 20% of a
+// CTA's time, is covered by the SM's other CTAs only in part.
 template <int DT>
 __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k) {
   using V = Vec<DT>;

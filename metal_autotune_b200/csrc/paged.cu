@@ -69,7 +69,10 @@ struct PlanArgs {
 // keeps the chunk's prefixes in shared memory; tokens, new pages and request
 // outputs are then shared out over the grid, each found by a binary search. A
 // token on a new page takes the page from the free list directly, so no CTA
-// reads a table entry that another one writes.
+// reads a table entry that another one writes. Latency bounds it: lengths,
+// scans, then a table or free-list entry for each token. 8 requests 3.6 us
+// (6.8 with 64-bit divisions), 4096 requests with 131072 token places 9.2 us,
+// where the 2.2 MB it moves would take 0.3.
 template <int kItems>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   constexpr int kPlanChunk = kPlanThreads * kItems;
@@ -283,11 +286,12 @@ __device__ __forceinline__ void store8(typename Elem<DT>::T* p, const float (&x)
   }
 }
 
-// Three rows to a group of lanes, two stages, 6 CTAs of 128 threads per SM (80 registers, 24 KB of ring each): 8192
-// tokens of 32/8 heads of 128 in 39.6 us. 5 CTAs with three stages 42.5; 7 or 8, whose registers spill, 58 and 62.
+// Three rows to a group of lanes, two stages, 5 CTAs of 128 threads per SM (91 registers, 24 KB of ring each): 8192
+// tokens of 32/8 heads of 128 with norms in 36.7 us = 5.5 TB/s, 84% of the copy rate. 6 CTAs, or a third stage, 38.6 to
+// 38.9; 4 with three stages 38.3.
 constexpr int kAppendRows = 3;
 constexpr int kAppendStages = 2;
-constexpr int kAppendCtas = 6;
+constexpr int kAppendCtas = 5;
 constexpr int kAppendThreads = 128;
 
 // cos and sin (times mscale) of one angle. The angle is reduced to a fraction
@@ -341,10 +345,12 @@ __device__ __forceinline__ uint4 pack(const float2* x) {
 // thread reads back only what it copied to shared memory itself: the rows of
 // the next STAGES - 1 items are always under way and need no barrier. The
 // angles of the next item are worked out, one by a thread, while this one's
-// rows arrive; one barrier per item hands them over. What limits it is
-// instructions, not memory: so two fp32 values to an instruction, and rows'
-// addresses, angles and weights come out of shared memory, which leaves
-// registers for six CTAs to an SM.
+// rows arrive; one barrier per item hands them over. What limited it was
+// instructions (0.48 a cycle, 724 for a warp's three rows: 72 us for the prompt
+// above) and then shared memory (75% busy with the angles read for each row,
+// 39.6 us): so two fp32 values to an instruction, a row's addresses and the
+// weights out of shared memory, the angles in registers for all rows. Norm and
+// rotation in fp32, rounded once.
 template <int DT, int LPR, bool TRAD, int ROWS, int STAGES>
 __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(const AppendArgs a) {
   using T = typename Elem<DT>::T;
@@ -359,7 +365,7 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(con
   };
   extern __shared__ __align__(16) uint8_t append_smem[];
   uint4(*ring)[ROWS][2][kAppendThreads] = reinterpret_cast<uint4(*)[ROWS][2][kAppendThreads]>(append_smem);
-  __shared__ __align__(16) float cos_of[2][128], sin_of[2][128], neg_sin_of[2][128];
+  __shared__ __align__(16) float cos_of[2][128], sin_of[2][128];
   __shared__ __align__(16) T weight[2][256];
   __shared__ __align__(16) Row rows[kGroup];
   __shared__ int64_t dst[2];
@@ -423,7 +429,6 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(con
       const float2 cs = cos_sin(pos, inv, a.mscale);
       cos_of[buf][tid] = cs.x;
       sin_of[buf][tid] = cs.y;
-      neg_sin_of[buf][tid] = -cs.y;
     }
     if (has_slot) dst[buf] = slot_offset(a, slot);
     if (next < a.T) {
@@ -440,6 +445,15 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(con
     if (t + step < a.T) hand_over(buf ^ 1, t + 2 * step);
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     const int64_t off = dst[buf], q_off = t * a.qo_st;
+    float2 c[P / 2], s[P / 2], ns[P / 2];
+    if (turned) {
+#pragma unroll
+      for (int e = 0; e < P / 2; ++e) {
+        c[e] = reinterpret_cast<const float2*>(&cos_of[buf][sub * P])[e];
+        s[e] = reinterpret_cast<const float2*>(&sin_of[buf][sub * P])[e];
+        ns[e] = make_float2(-s[e].x, -s[e].y);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const Row& w = rows[i * kRows + tid / LPR];
@@ -470,8 +484,6 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(con
           }
         }
         if (turned) {
-          const float2* c = reinterpret_cast<const float2*>(&cos_of[buf][sub * P]);
-          const float2* s = reinterpret_cast<const float2*>(&sin_of[buf][sub * P]);
           if constexpr (TRAD) {  // pairs within a piece: angles 0.. of the lane in x, then in y
 #pragma unroll
             for (int e = 0; e < P / 2; ++e) {
@@ -482,7 +494,6 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(con
               y[e] = make_float2(y[e].x * cy - y[e].y * sy, y[e].y * cy + y[e].x * sy);
             }
           } else {
-            const float2* ns = reinterpret_cast<const float2*>(&neg_sin_of[buf][sub * P]);
 #pragma unroll
             for (int e = 0; e < P / 2; ++e) {
               const float2 u = x[e], v = y[e];

@@ -316,10 +316,19 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, int64_t c0, int
 //
 // A warp that computes is fed by one that fetches, through a ring of stages:
 // finding the next keys' page and issuing their copies takes about as long as
-// computing on them does. The tensor instructions take 16 keys as their
-// rows and the query rows of a kv head as their 8 columns: S^T = K Q^T, then
-// O^T += V^T P^T, so up to 8 query heads of a kv head fill them without
-// padding, and an accumulator takes D/2 registers.
+// computing on them does (1050 and 720 cycles of a step of 16 keys when one
+// warp did both). The tensor instructions take 16 keys as their rows and the
+// query rows of a kv head as their 8 columns: S^T = K Q^T, then O^T += V^T P^T,
+// so up to 8 query heads of a kv head fill them without padding, and an
+// accumulator takes D/2 registers. The probabilities are rounded to 16 bits for
+// the product with V; maximum, sum and output stay in fp32.
+//
+// Memory bounds it where contexts are long: 4 flops a byte at 4 query heads to
+// a kv head. Heads of 128, 32/8, bf16, pages of 16: 64 requests of 64..8192
+// keys 78 us = 5.8 TB/s, 88% of the copy rate (92.5 us with one warp doing
+// both, by 16-byte copies); one of 131072 92 us, 89%. Few or short requests
+// wait for a chain of loads (lengths, page, keys: 2.6 us before the first
+// product) and the joins of split requests (1.5 us): one of 129 keys 6.1 us.
 template <int DT, int D, int R, int KEYS, int kStages, bool BOX, int kPerSm>
 __global__ void __launch_bounds__(kCtaThreads, kPerSm)
     paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
