@@ -143,13 +143,21 @@ struct Loader {
   }
 };
 
+// Keys and values are read once in a step and again only in the next one, after
+// all other layers': first to be evicted (32 requests of 1024 keys 29.8 -> 27.5
+// us, 256 of 1..512 27.8 -> 26.6), unless other rows of the head read them too.
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
-                                            int c3) {
+                                            int c3, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_addr(dst)),
-      "l"(map), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
       : "memory");
+}
+__device__ __forceinline__ uint64_t l2_evict_normal() {
+  uint64_t pol;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol));
+  return pol;
 }
 
 // The step's KEYS rows of K and V into stage memory, completing on `bar`. Rows
@@ -160,7 +168,7 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
 template <int D, int KEYS, bool BOX>
 __device__ __forceinline__ void load_step(const PagedParams& p, const CUtensorMap* kmap, const CUtensorMap* vmap,
                                           const Loader& c, int page, int key0, int lane, uint8_t* stage,
-                                          uint32_t* mask, uint64_t* bar) {
+                                          uint32_t* mask, uint64_t* bar, uint64_t policy) {
   const int key = key0 + (lane & (KEYS - 1));
   const bool there = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.num_pages);
   if (key < c.len && !there) report_status(0x702);
@@ -183,8 +191,8 @@ __device__ __forceinline__ void load_step(const PagedParams& p, const CUtensorMa
 #pragma unroll
         for (int half = 0; half < D / 64; ++half) {
           uint8_t* dst = stage + half * KEYS * 128 + g * 1024;
-          tma_load_4d(dst, kmap, bar, half * 64, slot, c.hk, pages[g]);
-          tma_load_4d(dst + KEYS * D * 2, vmap, bar, half * 64, slot, c.hk, pages[g]);
+          tma_load_4d(dst, kmap, bar, half * 64, slot, c.hk, pages[g], policy);
+          tma_load_4d(dst + KEYS * D * 2, vmap, bar, half * 64, slot, c.hk, pages[g], policy);
         }
       }
     }
@@ -478,12 +486,13 @@ __global__ void __launch_bounds__(kCtaThreads, kPerSm)
     ld.ahead_b = -1;
     ld.ahead_base = -1;
     int64_t step = 0;
+    const uint64_t policy = p.RB > 1 ? l2_evict_normal() : l2_evict_first();
     while (ld.left > 0) {
       const int key0 = ld.t * keys + first;
       const int page = ld.page_of<KEYS>(p, key0, heads, lane);
       if (step >= kStages && !mbar_wait_warp(&sm.empty[warp][at], phase ^ 1, &sm.abort, 0x704)) return;  // reported
       load_step<D, KEYS, BOX>(p, &kmap, &vmap, ld, page, key0, lane, stages + at * Smem::kStageBytes, &sm.mask[warp][at],
-                        &sm.full[warp][at]);
+                              &sm.full[warp][at], policy);
       if (ld.advance(p, heads, keys)) {  // another request: its first window has come in, or has not
         const bool come = ld.ahead_b == ld.b && ld.ahead_base == 0;
         ld.win = ld.ahead;
@@ -847,7 +856,6 @@ int mt_paged_sdpa_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* 
   // the copy engine where pages hold whole boxes and its strides can express the cache
   const int64_t bytes[3] = {slot_stride * 2, head_stride * 2, page_stride * 2};
   const int64_t extent[3] = {page_size, Hkv, num_pages};
-  p.box_rows = D == 64 && page_size % 32 == 0 ? 32 : page_size % 16 == 0 ? 16 : 8;
   bool box = page_size % 8 == 0 && num_pages > 0;
   uint64_t dims[4] = {(uint64_t)D}, strides[3];
   for (int i = 0; i < 3; ++i) {
@@ -855,6 +863,11 @@ int mt_paged_sdpa_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* 
     strides[i] = extent[i] > 1 ? (uint64_t)bytes[i] : 16;
     box = box && extent[i] < (1ll << 32) && (extent[i] == 1 || (bytes[i] > 0 && bytes[i] < (1ll << 40)));
   }
+  // Steps of 32 keys for heads of 64, and for heads of 128 where there are few units: then one CTA to an SM, fewer parts
+  // to join and more bytes to a copy of the copy engine (without it, 15.4 -> 16.6 us for 16 requests of 64..2048). 64 requests of 64..8192 keys (512 units) 77.2 -> 75.6 us, four of 4096 18.9 ->
+  // 16.9, one of 131072 90.6 -> 87.8; but 128 of 64..2048 (1024 units) 55.0 -> 58.4, 256 of 1..512 26.7 -> 29.1.
+  const bool wide = D == 64 || (R == 8 && box && B * Hkv * RB <= 512);
+  p.box_rows = wide && page_size % 32 == 0 ? 32 : page_size % 16 == 0 ? 16 : 8;
   CUtensorMap kmap = {}, vmap = {};
   if (box) {
     const uint32_t shape[4] = {64, (uint32_t)p.box_rows, 1, 1};
@@ -884,6 +897,7 @@ int mt_paged_sdpa_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* 
       return R == 16 ? with(Int<16>(), Int<32>(), Int<2>(), Int<2>()) : with(Int<8>(), Int<32>(), Int<3>(), Int<2>());
     else
       return R == 16  ? with(Int<16>(), Int<16>(), Int<4>(), Int<1>())
+             : wide   ? with(Int<8>(), Int<32>(), Int<3>(), Int<1>())
              : G <= 4 ? with(Int<8>(), Int<16>(), Int<3>(), Int<2>())
                       : with(Int<8>(), Int<16>(), Int<2>(), Int<2>());
   };

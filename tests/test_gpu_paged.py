@@ -330,6 +330,11 @@ ATTEND = [
     ([(37 * i) % 301 for i in range(600)], 8, 8, 64, 12, "f16", "nhd"),
     ([400 + (91 * i) % 300 for i in range(300)], 6, 1, 128, 8, "bf16", "nhd"),
     ([2000, 0, 1, 900, 4097], 48, 4, 128, 32, "f16", "hnd"),  # 12 rows a head
+    ([31, 32, 33, 95, 1000, 5000], 12, 2, 128, 32, "bf16", "hnd"),   # few units: steps of 32 keys, 6 rows a head
+    ([7, 0, 40, 129, 3000], 4, 2, 128, 8, "f16", "nhd"),
+    ([40, 777, 5], 4, 1, 128, 9, "bf16", "hnd"),
+    ([20 + i for i in range(140)], 16, 4, 128, 48, "bf16", "nhd"),   # more units: steps of 16
+    ([1000, 33, 64], 8, 1, 64, 32, "bf16", "hnd"),
 ]
 
 
