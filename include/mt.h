@@ -601,7 +601,8 @@ int mt_rope_paged_append(
  * head h / (Hq / Hkv). q and o [B, Hq, D] with strides (request, head), D
  * contiguous (q rows 4-byte, o rows 8-byte aligned); D = 64 or 128; bf16 or
  * f16; any page_size. A length of 0 (or less) gives zeros; lengths past
- * max_pages * page_size are cut there. A page id outside the cache hides its
+ * max_pages * page_size are cut there (B * max_pages * page_size below 2^35 rows
+ * in all, MT_ERR_UNSUPPORTED beyond). A page id outside the cache hides its
  * keys and is reported through the device status. Scores, softmax sums and
  * outputs are accumulated in fp32, the probabilities rounded to dtype for the
  * product with v. The work is split over the keys, so a request's sums may

@@ -3,6 +3,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_common.cuh"
 
@@ -11,16 +12,18 @@ namespace cg = cooperative_groups;
 namespace mt {
 namespace {
 
-// 5 CTAs of 256 threads per SM, 64 bytes in flight a thread: 2048 x 151936 bf16 with 20 alternatives 126 us; 4 CTAs
-// 133, 6 (40 registers, spilled) 165, 3 vectors in flight 133, 3 CTAs of 512 threads 142.
+// 5 CTAs of 256 threads per SM, 64 bytes in flight a thread: 2048 x 151936 bf16 with 20 alternatives 126 us when it was
+// chosen (121 now); 4 CTAs 133, 6 (40 registers, spilled) 165, 3 vectors in flight 133, 3 CTAs of 512 threads 142.
 constexpr int kThreads = 256;
 constexpr int kCtasPerSm = 5;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;    // one key per lane
 constexpr int kMaxSplit = 8;   // CTAs to a row
 static_assert(kMaxSplit <= kWarps, "the first CTA joins a list per warp");
-constexpr int kUnroll = 4;     // 16-byte loads a thread has in flight (a batch)
-constexpr int kBatch = kThreads * kUnroll;
+// 16-byte loads a thread has in flight (a batch). Rows that several CTAs share leave a thread few vectors (151936 values
+// over 8 CTAs 9 or 10), so twice as many at once, at 4 CTAs per SM, whose registers that takes: one row 8.4 -> 8.1 us,
+// 256 rows 28.0 -> 25.2. (12 at 3 CTAs: 8.4 and 29.1.)
+constexpr int kUnrollMany = 4, kUnrollFew = 8, kCtasPerSmFew = 4;
 constexpr int kGroups = 64;    // groups of threads whose maxima bound the k-th largest value
 constexpr int kEntries = 32;   // maxima of its batches that a thread keeps
 constexpr int kCap = 2048;     // candidates kept before the exact form takes over
@@ -136,6 +139,14 @@ __device__ __forceinline__ uint64_t sort_up(uint64_t a, int lane) {
   for (int n = 2; n <= 32; n <<= 1)
 #pragma unroll
     for (int o = n >> 1; o > 0; o >>= 1) a = pick(a, o, ((lane & o) == 0) == ((lane & n) != 0 && n < 32));
+  return a;
+}
+// any order -> falling
+__device__ __forceinline__ uint64_t sort_down(uint64_t a, int lane) {
+#pragma unroll
+  for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+    for (int o = n >> 1; o > 0; o >>= 1) a = pick(a, o, ((lane & o) == 0) == ((lane & n) == 0 || n == 32));
   return a;
 }
 // falling list + rising batch -> falling list of the 32 largest
@@ -284,10 +295,10 @@ __device__ __noinline__ void exact_slice(Smem& sm, const Part<DT>& p, int top_k)
 // 223 us when the bound came from the row's beginning and candidates left the
 // loop one by one). The loop runs at the copy rate; what follows it, 20% of a
 // CTA's time, is covered by the SM's other CTAs only in part.
-template <int DT>
+template <int DT, int kUnroll>
 __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k) {
   using V = Vec<DT>;
-  constexpr int E = V::E;
+  constexpr int E = V::E, kBatch = kThreads * kUnroll;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = static_cast<int>(p.v1 - p.v0);                   // an index is below 2^31
   const uint32_t i0 = static_cast<uint32_t>(p.body + p.v0 * E);  // index of the slice's first value
@@ -314,7 +325,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
   }
   float top = 0.f;  // the thread's largest value, in vector `at` (the first that holds it)
   int at = -1, entry = 0, in_entry = 0;
-  auto take_batch = [&](const uint4 (&r)[kUnroll], int j0) {
+  auto take_batch = [&](const uint4 (&r)[kUnroll], int j0, int left) {  // left: vectors from the warp's first on
     float m[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) m[u] = V::vmax(r[u]);
@@ -340,15 +351,17 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
     if (mb > a.ref + 1.0f) a.raise(mb);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
+      if (u * kThreads < left) {
 #pragma unroll
-      for (int q = 0; q < E / 2; ++q) a.add(V::pair(r[u], q));
+        for (int q = 0; q < E / 2; ++q) a.add(V::pair(r[u], q));
+      }
   };
   int j0 = 0;
   for (; j0 + kBatch <= n; j0 += kBatch) {
     uint4 r[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) r[u] = __ldcs(v + j0 + u * kThreads + tid);
-    take_batch(r, j0);
+    take_batch(r, j0, kBatch);
   }
   if (j0 < n) {
     uint4 r[kUnroll];
@@ -357,7 +370,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
       const int j = j0 + u * kThreads + tid;
       r[u] = j < n ? __ldcs(v + j) : none;
     }
-    take_batch(r, j0);
+    take_batch(r, j0, n - j0 - warp * 32);
   }
 
   // the bound: the k-th largest of the groups' maxima
@@ -400,7 +413,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
     for (int o = 1; o < kPer; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
     if (tid % kPer == 0 && rank == top_k - 1) sm.thr_key = mine;
   }
-  if (warp == 0) {
+  auto join_sums = [&]() {  // a warp
     const float mr = lane < kWarps ? sm.red[0][lane] : -INFINITY;
     const float mb = warp_max(mr);
     d = lane < kWarps ? mr - mb : 0.f;
@@ -416,10 +429,13 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
       // the largest value alone adds over 1/2, unless it lies below kFloor or the row holds NaN or +inf
       sm.exact = !(s >= 0.25f && s < INFINITY && t == t);
     }
+  };
+  if (top_k == 0) {
+    if (warp == 0) join_sums();
+    __syncthreads();
+    return !sm.exact;
   }
   __syncthreads();
-  if (sm.exact) return false;
-  if (top_k == 0) return true;
   const uint64_t thr_key = sm.thr_key;
   const float thr = key_value(thr_key);  // NaN where fewer than k groups hold anything: all count
   auto push = [&](uint64_t key) {
@@ -437,6 +453,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
   int* hits = reinterpret_cast<int*>(sm.lists);
   constexpr int kHits = sizeof(sm.lists) / sizeof(int);
   const int span = per * kBatch;
+  if (warp == kWarps - 1) join_sums();
   for (int e = 0; e * span < n; ++e)
     if (!(__bfloat162float(sm.batch_max[e][tid]) < thr)) {
       const int h = atomicAdd(&sm.hits, 1);
@@ -455,11 +472,13 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
   }
   if (extra_i >= 0) push(top_key(extra, static_cast<uint32_t>(extra_i)));
   __syncthreads();
-  if (sm.count > kCap) return false;
+  if (sm.exact || sm.count > kCap) return false;
   // top 32 of the candidates: batches of 32 sorted by the warps, their lists joined in pairs
   const int c = sm.count;
   uint64_t list = 0;
-  for (int b = warp * 32; b < c; b += kThreads) list = take(list, sort_up(b + lane < c ? sm.buf[b + lane] : 0, lane), lane);
+  if (warp * 32 < c) list = sort_down(warp * 32 + lane < c ? sm.buf[warp * 32 + lane] : 0, lane);
+  for (int b = warp * 32 + kThreads; b < c; b += kThreads)
+    list = take(list, sort_up(b + lane < c ? sm.buf[b + lane] : 0, lane), lane);
   list = join_lists(sm, list, min(kWarps, (c + 31) >> 5));
   if (warp == 0) sm.out.list[lane] = list;
   return true;
@@ -467,8 +486,8 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
 
 // A row per CTA, or `split` CTAs of a cluster per row where there are few rows;
 // the first joins the others' sums and lists through distributed shared memory.
-template <int DT>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const LogprobArgs a) {
+template <int DT, int kUnroll, int kPerSm>
+__global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const LogprobArgs a) {
   using T = typename Elem<DT>::T;
   constexpr int E = Vec<DT>::E;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -489,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const Lo
   p.v1 = nvec * (rank + 1) >> a.split_bits;
   p.head = rank == 0 ? static_cast<int>(p.body) : 0;
   p.tail = rank == 0 ? static_cast<int>(a.V - p.tail0) : 0;
-  if (!one_pass<DT>(sm, p, a.top_k)) exact_slice<DT>(sm, p, a.top_k);
+  if (!one_pass<DT, kUnroll>(sm, p, a.top_k)) exact_slice<DT>(sm, p, a.top_k);
   __syncthreads();
   double m = sm.out.m;
   float s = sm.out.s, t = sm.out.t;
@@ -566,19 +585,23 @@ extern "C" int mt_token_logprobs(const void* logits, int64_t row_stride, const i
   int sms = 148;
   if (int rc = device_sm_count(&sms)) return rc;
   int bits = 0;
-  while ((2 << bits) <= kMaxSplit && (R << (bits + 1)) <= kCtasPerSm * sms && (V >> (bits + 1)) >= 4096) ++bits;
+  while ((2 << bits) <= kMaxSplit && (R << (bits + 1)) <= kCtasPerSmFew * sms && (V >> (bits + 1)) >= 4096) ++bits;
   const LogprobArgs a = {logits, row_stride, V, tokens, top_k, bits, logprob, entropy, lse, top_ids, top_logprobs};
   // where there are fewer CTAs than fit, as much shared memory as leaves every SM its share of them: clusters are else
   // packed onto some of the SMs
   // (and a little more room for clusters of 8, which do not come out even over the SMs)
   const int64_t ctas = R << bits, share = ((bits == 3 ? ctas + ctas / 4 : ctas) + sms - 1) / sms;
   size_t smem = sizeof(Smem);
-  if (share < kCtasPerSm) smem = std::max(smem, static_cast<size_t>(228 * 1024 / share - 1024) / 1024 * 1024);
+  if (share < (bits > 0 ? kCtasPerSmFew : kCtasPerSm)) smem = std::max(smem, static_cast<size_t>(228 * 1024 / share - 1024) / 1024 * 1024);
   auto run = [&](auto kern) -> int {
     if (int e = ensure_smem(kern, 227 * 1024)) return e;
     return launch_cluster(kern, dim3((unsigned)(R << bits)), dim3(kThreads), smem, 1 << bits, (cudaStream_t)stream, a);
   };
-  return dtype == MT_BF16  ? run(logprobs_kernel<MT_BF16>)
-         : dtype == MT_F16 ? run(logprobs_kernel<MT_F16>)
-                           : run(logprobs_kernel<MT_F32>);
+  auto pick_unroll = [&](auto type) -> int {
+    constexpr int DT = decltype(type)::value;
+    return bits > 0 ? run(logprobs_kernel<DT, kUnrollFew, kCtasPerSmFew>) : run(logprobs_kernel<DT, kUnrollMany, kCtasPerSm>);
+  };
+  return dtype == MT_BF16  ? pick_unroll(std::integral_constant<int, MT_BF16>())
+         : dtype == MT_F16 ? pick_unroll(std::integral_constant<int, MT_F16>())
+                           : pick_unroll(std::integral_constant<int, MT_F32>());
 }

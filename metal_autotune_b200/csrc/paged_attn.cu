@@ -333,10 +333,10 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, int64_t c0, int
 //
 // Memory bounds it where contexts are long: 4 flops a byte at 4 query heads to
 // a kv head. Heads of 128, 32/8, bf16, pages of 16: 64 requests of 64..8192
-// keys 78 us = 5.8 TB/s, 88% of the copy rate (92.5 us with one warp doing
-// both, by 16-byte copies); one of 131072 92 us, 89%. Few or short requests
+// keys 75 us = 6.0 TB/s, 92% of the copy rate (92.5 us with one warp doing
+// both, by 16-byte copies); one of 131072 87 us, 94%. Few or short requests
 // wait for a chain of loads (lengths, page, keys: 2.6 us before the first
-// product) and the joins of split requests (1.5 us): one of 129 keys 6.1 us.
+// product) and the joins of split requests (1.5 us): one of 129 keys 6.2 us.
 template <int DT, int D, int R, int KEYS, int kStages, bool BOX, int kPerSm>
 __global__ void __launch_bounds__(kCtaThreads, kPerSm)
     paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -864,8 +864,9 @@ int mt_paged_sdpa_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* 
     box = box && extent[i] < (1ll << 32) && (extent[i] == 1 || (bytes[i] > 0 && bytes[i] < (1ll << 40)));
   }
   // Steps of 32 keys for heads of 64, and for heads of 128 where there are few units: then one CTA to an SM, fewer parts
-  // to join and more bytes to a copy of the copy engine (without it, 15.4 -> 16.6 us for 16 requests of 64..2048). 64 requests of 64..8192 keys (512 units) 77.2 -> 75.6 us, four of 4096 18.9 ->
-  // 16.9, one of 131072 90.6 -> 87.8; but 128 of 64..2048 (1024 units) 55.0 -> 58.4, 256 of 1..512 26.7 -> 29.1.
+  // to join and more bytes to a copy of the copy engine. 64 requests of 64..8192 keys (512 units) 77.2 -> 75.6 us, four
+  // of 4096 18.9 -> 16.9, one of 131072 90.6 -> 87.8; but 128 of 64..2048 (1024 units) 55.0 -> 58.4, 256 of 1..512 26.7
+  // -> 29.1, and by 16-byte copies 16 of 64..2048 15.4 -> 16.6.
   const bool wide = D == 64 || (R == 8 && box && B * Hkv * RB <= 512);
   p.box_rows = wide && page_size % 32 == 0 ? 32 : page_size % 16 == 0 ? 16 : 8;
   CUtensorMap kmap = {}, vmap = {};

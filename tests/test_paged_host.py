@@ -79,6 +79,7 @@ def test_attend_refuses(mt):
     refused(mt, attend(page=0), -1, b"page_size=0")
     refused(mt, attend(stride=4), -1, b"table stride=4")
     refused(mt, attend(lens=None), -1, b"null pointer")
+    refused(mt, attend(B=1 << 16, width=1 << 16, stride=1 << 16), -2, b"2^35 rows")
     refused(mt, attend(ss=100), -1, b"16-byte aligned")
     refused(mt, attend(ws=None), -3, b"needs a workspace")
     refused(mt, attend(nb=need - 1), -3, b"needs a workspace")
