@@ -11,8 +11,6 @@ namespace {
 // request's rows start) and new pages (which free pages it gets). Both are
 // sums of non-negative numbers that saturate at INT32_MAX, so adding in any
 // grouping gives the same result and nothing overflows, whatever the lengths.
-constexpr int kPlanThreads = 512;
-constexpr int kPlanItems = 8;  // requests to a thread at a time; 1 where there are no more than threads
 constexpr int kPlanMax = 0x7fffffff;
 
 __device__ __forceinline__ int sat_add(int a, int b) {
@@ -21,11 +19,12 @@ __device__ __forceinline__ int sat_add(int a, int b) {
 }
 
 struct PlanScan {
-  int warp_sum[kPlanThreads / 32];
+  int warp_sum[32];
 };
 
 // Inclusive saturating scan of `own` over the block, plus `carry`; returns the
 // exclusive prefix of this thread and the block's total through `total`.
+template <int kThreads>
 __device__ __forceinline__ int plan_scan(int own, int carry, PlanScan& sm, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int inc = own;
@@ -38,14 +37,14 @@ __device__ __forceinline__ int plan_scan(int own, int carry, PlanScan& sm, int& 
   if (lane == 0) before = 0;
   if (lane == 31) sm.warp_sum[warp] = inc;
   __syncthreads();
-  int w = lane < kPlanThreads / 32 ? sm.warp_sum[lane] : 0;
+  int w = lane < kThreads / 32 ? sm.warp_sum[lane] : 0;
 #pragma unroll
-  for (int o = 1; o < kPlanThreads / 32; o <<= 1) {
+  for (int o = 1; o < kThreads / 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, w, o);
     if (lane >= o) w = sat_add(w, u);
   }
   const int prev = warp > 0 ? __shfl_sync(0xffffffffu, w, warp - 1) : 0;
-  total = sat_add(carry, __shfl_sync(0xffffffffu, w, kPlanThreads / 32 - 1));
+  total = sat_add(carry, __shfl_sync(0xffffffffu, w, kThreads / 32 - 1));
   __syncthreads();  // sm.warp_sum is written again by the next scan
   return sat_add(carry, sat_add(prev, before));
 }
@@ -71,13 +70,14 @@ struct PlanArgs {
 // token on a new page takes the page from the free list directly, so no CTA
 // reads a table entry that another one writes. Latency bounds it: lengths,
 // scans, then a table or free-list entry for each token. 8 requests 3.6 us
-// (6.8 with 64-bit divisions), 4096 requests with 131072 token places 9.2 us,
-// where the 2.2 MB it moves would take 0.3.
-template <int kItems>
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
-  constexpr int kPlanChunk = kPlanThreads * kItems;
-  // a place in eight is left out, so that threads with eight requests each do not meet in a bank
-  auto pad = [](int r) { return r + (r >> 3); };
+// (6.8 with 64-bit divisions), 4096 requests with 131072 token places 8.9 us
+// (9.2 with 512 threads of eight requests, 9.8 while those met in shared-memory
+// banks), where the 2.2 MB it moves would take 0.3.
+template <int kThreads, int kItems>
+__global__ void __launch_bounds__(kThreads) plan_kernel(const PlanArgs a) {
+  constexpr int kPlanChunk = kThreads * kItems;
+  // a place in kItems is left out, so that threads with so many requests each do not meet in a bank
+  auto pad = [](int r) { return kItems == 1 ? r : r + r / kItems; };
   extern __shared__ int plan_smem[];
   int* tok_end = plan_smem;                  // inclusive sums of new tokens
   int* page_end = tok_end + pad(kPlanChunk);  // inclusive sums of new pages
@@ -85,7 +85,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   __shared__ PlanScan scan;
   __shared__ int red[3];
   griddep_wait();
-  griddep_launch();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int ps = a.page.d;
   const int n_free = static_cast<int>(a.n_free);
@@ -103,11 +102,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     alignas(16) int ctx[kItems], fresh[kItems];
     int need[kItems];
     int own = 0;
-    if (kItems == 8 && vec && tid * 8 + 8 <= n) {
+    if (kItems % 4 == 0 && vec && tid * kItems + kItems <= n) {
 #pragma unroll
-      for (int i = 0; i < kItems; i += 4) {
-        *reinterpret_cast<int4*>(ctx + i) = *reinterpret_cast<const int4*>(a.ctx + r0 + tid * 8 + i);
-        *reinterpret_cast<int4*>(fresh + i) = *reinterpret_cast<const int4*>(a.fresh + r0 + tid * 8 + i);
+      for (int i = 0; i + 3 < kItems; i += 4) {
+        *reinterpret_cast<int4*>(ctx + i) = *reinterpret_cast<const int4*>(a.ctx + r0 + tid * kItems + i);
+        *reinterpret_cast<int4*>(fresh + i) = *reinterpret_cast<const int4*>(a.fresh + r0 + tid * kItems + i);
       }
     } else {
 #pragma unroll
@@ -124,7 +123,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
       own = sat_add(own, fresh[i]);
     }
     int tok_total, page_total;
-    int t = plan_scan(own, tok_base, scan, tok_total);
+    int t = plan_scan<kThreads>(own, tok_base, scan, tok_total);
     own = 0;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
@@ -137,7 +136,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
       own = sat_add(own, max(need[i], 0));
       tok_end[pad(r)] = t;
     }
-    int p = plan_scan(own, page_base, scan, page_total);
+    int p = plan_scan<kThreads>(own, page_base, scan, page_total);
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int r = tid * kItems + i;
@@ -157,8 +156,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     __syncthreads();
     // new pages of this chunk's admitted requests
     const int page_last = min(page_total, avail);
-    for (int64_t e = page_base + static_cast<int64_t>(blockIdx.x) * kPlanThreads + tid; e < page_last;
-         e += static_cast<int64_t>(gridDim.x) * kPlanThreads) {
+    for (int64_t e = page_base + static_cast<int64_t>(blockIdx.x) * kThreads + tid; e < page_last;
+         e += static_cast<int64_t>(gridDim.x) * kThreads) {
       int lo = 0, hi = n - 1;  // first request with page_end > e
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
@@ -172,8 +171,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     }
     // tokens of this chunk, two of a thread's at a time so that their searches and loads overlap
     const int64_t tok_last = tok_total < a.cap ? tok_total : a.cap;
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * kPlanThreads;
-    for (int64_t k0 = tok_base + static_cast<int64_t>(blockIdx.x) * kPlanThreads + tid; k0 < tok_last; k0 += 2 * stride) {
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
+    for (int64_t k0 = tok_base + static_cast<int64_t>(blockIdx.x) * kThreads + tid; k0 < tok_last; k0 += 2 * stride) {
       int at[2] = {0, 0}, block[2], page[2];
       int64_t pos[2];
 #pragma unroll 1
@@ -208,8 +207,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     page_base = page_total;
     __syncthreads();  // the prefixes are overwritten by the next chunk
   }
-  for (int64_t k = tok_base + static_cast<int64_t>(blockIdx.x) * kPlanThreads + tid; k < a.cap;
-       k += static_cast<int64_t>(gridDim.x) * kPlanThreads) {
+  griddep_launch();  // not at the top: the next kernel's CTAs beside these cost 1.7 us of 11.6 in a stream
+  for (int64_t k = tok_base + static_cast<int64_t>(blockIdx.x) * kThreads + tid; k < a.cap;
+       k += static_cast<int64_t>(gridDim.x) * kThreads) {
     a.positions[k] = 0;
     a.token_seq[k] = -1;
     a.slots[k] = -1;
@@ -648,14 +648,15 @@ int mt_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int64_t B, i
   if (int rc = device_sm_count(&sms)) return rc;
   const PlanArgs a = {ctx_lens, new_lens, B, block_table, table_stride, max_pages, free_pages, free_head, n_free,
                       FastDiv::of((int)page_size), token_cap, seq_lens, query_start, positions, token_seq, slots, counts};
-  const int64_t want = (token_cap + kPlanThreads - 1) / kPlanThreads;
-  const int64_t grid = want < 1 ? 1 : want < sms ? want : sms;
-  auto run = [&](auto kern, int items) -> int {
-    const size_t smem = 3 * sizeof(int) * (kPlanThreads * items + kPlanThreads * items / 8);
+  auto run = [&](auto kern, int threads, int items) -> int {
+    const int64_t want = (token_cap + threads - 1) / threads;
+    const int64_t grid = want < 1 ? 1 : want < sms ? want : sms;
+    const size_t smem = 3 * sizeof(int) * (threads * items + threads);
     if (int rc = ensure_smem(kern, smem)) return rc;
-    return launch(kern, dim3((unsigned)grid), dim3(kPlanThreads), smem, (cudaStream_t)stream, a);
+    return launch(kern, dim3((unsigned)grid), dim3(threads), smem, (cudaStream_t)stream, a);
   };
-  return B <= kPlanThreads ? run(plan_kernel<1>, 1) : run(plan_kernel<kPlanItems>, kPlanItems);
+  // one request to a thread where there are few, else four to each of 1024, 4096 scanned at a time
+  return B <= 512 ? run(plan_kernel<512, 1>, 512, 1) : run(plan_kernel<1024, 4>, 1024, 4);
 }
 
 int mt_rope_paged_append(const void* q, const void* k, const void* v, int64_t q_st, int64_t q_sh, int64_t k_st,
