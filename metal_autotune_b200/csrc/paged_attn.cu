@@ -336,7 +336,7 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, int64_t c0, int
 // keys 75 us = 6.0 TB/s, 92% of the copy rate (92.5 us with one warp doing
 // both, by 16-byte copies); one of 131072 87 us, 94%. Few or short requests
 // wait for a chain of loads (lengths, page, keys: 2.6 us before the first
-// product) and the joins of split requests (1.5 us): one of 129 keys 6.2 us.
+// product) and the joins of split requests (1.5 us): one of 129 keys 5.8 us.
 template <int DT, int D, int R, int KEYS, int kStages, bool BOX, int kPerSm>
 __global__ void __launch_bounds__(kCtaThreads, kPerSm)
     paged_kernel(const PagedParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -580,15 +580,6 @@ __global__ void __launch_bounds__(kCtaThreads, kPerSm)
       uint8_t* stage = stages + at * Smem::kStageBytes;
       const uint32_t kaddr = smem_addr(stage), vaddr = kaddr + KEYS * D * 2;
       if (mask != 0) {
-        if (mask != kAll) {  // rows of V without a key are zeros, not what the page or the stage holds there
-          for (int i = lane; i < KEYS * (D / 8); i += 32) {
-            const int row = i / (D / 8);
-            if (!((mask >> row) & 1))
-              *reinterpret_cast<uint4*>(stage + KEYS * D * 2 + swz<KEYS>(row, i % (D / 8))) = make_uint4(0, 0, 0, 0);
-          }
-          if (BOX) fence_proxy_async_shared();
-          __syncwarp();
-        }
         constexpr int CH = NK == 1 ? 2 : 1;  // chains over the head for a block of keys, added at the end
         float s[NK][NB][CH][4];
 #pragma unroll
@@ -659,16 +650,34 @@ __global__ void __launch_bounds__(kCtaThreads, kPerSm)
             pb[kb][j][1] = transpose8(pack2<DT>(e2, e3));
           }
         }
+        // O^T += V^T P^T. Rows of V without a key count as zeros, whatever the page or the stage holds there (a probability
+        // of 0 would not clear a NaN): their fragments are masked in registers; zeros written to the stage instead
+        // made one request of 129 keys 6.3 us for 5.8, 2048 of one key 46.4 for 42.8. Whole steps have a loop of their own.
+        auto product = [&](auto part) {
 #pragma unroll
-        for (int kb = 0; kb < NK; ++kb)
+          for (int kb = 0; kb < NK; ++kb) {
+            // this lane's keys: 16 kb + 2 (lane % 4) and the next, + 8 in `upper`
+            const uint32_t bits = mask >> (kb * 16 + (lane & 3) * 2);
+            const uint32_t lower = ((bits & 1) ? 0xffffu : 0u) | ((bits & 2) ? 0xffff0000u : 0u);
+            const uint32_t upper = ((bits & 0x100) ? 0xffffu : 0u) | ((bits & 0x200) ? 0xffff0000u : 0u);
 #pragma unroll
-          for (int n = 0; n < KS; ++n) {
-            uint32_t a[4];
-            ldsm_x4_t(vaddr + swz<KEYS>(kb * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * n + ((lane >> 3) & 1)), a[0], a[1],
-                      a[2], a[3]);
+            for (int n = 0; n < KS; ++n) {
+              uint32_t a[4];
+              ldsm_x4_t(vaddr + swz<KEYS>(kb * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * n + ((lane >> 3) & 1)), a[0], a[1],
+                        a[2], a[3]);
+              if constexpr (decltype(part)::value) {
+                a[0] &= lower;
+                a[1] &= lower;
+                a[2] &= upper;
+                a[3] &= upper;
+              }
 #pragma unroll
-            for (int j = 0; j < NB; ++j) mma16816<DT>(acc[n][j], a, pb[kb][j][0], pb[kb][j][1]);
+              for (int j = 0; j < NB; ++j) mma16816<DT>(acc[n][j], a, pb[kb][j][0], pb[kb][j][1]);
+            }
           }
+        };
+        if (mask == kAll) product(std::false_type());
+        else product(std::true_type());
       }
       __syncwarp();
       if (dead) continue;  // the stage stays taken: the warp that fetches gives up too
