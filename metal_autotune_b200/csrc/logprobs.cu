@@ -13,7 +13,7 @@ namespace mt {
 namespace {
 
 // 5 CTAs of 256 threads per SM, 64 bytes in flight a thread: 2048 x 151936 bf16 with 20 alternatives 126 us when it was
-// chosen (121 now); 4 CTAs 133, 6 (40 registers, spilled) 165, 3 vectors in flight 133, 3 CTAs of 512 threads 142.
+// chosen (120 now); 4 CTAs 133, 6 (40 registers, spilled) 165, 3 vectors in flight 133, 3 CTAs of 512 threads 142.
 constexpr int kThreads = 256;
 constexpr int kCtasPerSm = 5;
 constexpr int kWarps = kThreads / 32;
@@ -45,17 +45,26 @@ __device__ __forceinline__ int key_index(uint64_t key) {
   return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
 }
 
-// A 16-byte vector of logits: its maximum (NaN skipped where there is another
+// A 16-byte vector of logits: its maxima (NaN skipped where there is another
 // value), its values as they are, and its values with -inf raised to a finite
-// bound far below kFloor, NaN kept: 0 * -inf never arises in the sums.
-template <int DT> struct Vec;
-template <> struct Vec<MT_BF16> {
+// bound far below kFloor, NaN kept: 0 * -inf never arises in the sums. The
+// maxima of 16-bit values stay two to a register until a batch's are joined
+// (32 rows 11.8 -> 11.6 us, 256 25.2 -> 24.6, 2048 121.2 -> 120.3).
+template <typename T2> struct Vec16 {
   static constexpr int E = 8;
-  static __device__ __forceinline__ float vmax(const uint4& u) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-    return fmaxf(f.x, f.y);
+  using Max = T2;
+  static __device__ __forceinline__ Max maxima(const uint4& u) {
+    const T2* h = reinterpret_cast<const T2*>(&u);
+    return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
   }
+  static __device__ __forceinline__ Max larger(Max a, Max b) { return __hmax2(a, b); }
+  static __device__ __forceinline__ Max across(Max a) { return __hmax2(a, __lowhigh2highlow(a)); }  // in both halves
+  static __device__ __forceinline__ bool holds(Max a, Max whole) { return __heq2_mask(a, whole) != 0; }
+  static __device__ __forceinline__ float value(Max whole) { return __low2float(whole); }
+};
+template <int DT> struct Vec;
+template <> struct Vec<MT_BF16> : Vec16<__nv_bfloat162> {
+  static __device__ __forceinline__ __nv_bfloat16 round_up(Max whole) { return __low2bfloat16(whole); }
   static __device__ __forceinline__ float raw(const uint4& u, int e) {
     return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(&u)[e]);
   }
@@ -64,13 +73,8 @@ template <> struct Vec<MT_BF16> {
     return __bfloat1622float2(__hmax2_nan(reinterpret_cast<const __nv_bfloat162*>(&u)[p], low));
   }
 };
-template <> struct Vec<MT_F16> {
-  static constexpr int E = 8;
-  static __device__ __forceinline__ float vmax(const uint4& u) {
-    const __half2* h = reinterpret_cast<const __half2*>(&u);
-    const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-    return fmaxf(f.x, f.y);
-  }
+template <> struct Vec<MT_F16> : Vec16<__half2> {
+  static __device__ __forceinline__ __nv_bfloat16 round_up(Max whole) { return __float2bfloat16_ru(value(whole)); }
   static __device__ __forceinline__ float raw(const uint4& u, int e) {
     return __half2float(reinterpret_cast<const __half*>(&u)[e]);
   }
@@ -81,14 +85,20 @@ template <> struct Vec<MT_F16> {
 };
 template <> struct Vec<MT_F32> {
   static constexpr int E = 4;
+  using Max = float;
   static __device__ __forceinline__ float max_nan(float a, float b) {
     float d;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
   }
-  static __device__ __forceinline__ float vmax(const uint4& u) {
+  static __device__ __forceinline__ Max maxima(const uint4& u) {
     return fmaxf(fmaxf(raw(u, 0), raw(u, 1)), fmaxf(raw(u, 2), raw(u, 3)));
   }
+  static __device__ __forceinline__ Max larger(Max a, Max b) { return fmaxf(a, b); }
+  static __device__ __forceinline__ Max across(Max a) { return a; }
+  static __device__ __forceinline__ bool holds(Max a, Max whole) { return a == whole; }
+  static __device__ __forceinline__ float value(Max whole) { return whole; }
+  static __device__ __forceinline__ __nv_bfloat16 round_up(Max whole) { return __float2bfloat16_ru(whole); }
   static __device__ __forceinline__ float raw(const uint4& u, int e) {
     return reinterpret_cast<const float*>(&u)[e];
   }
@@ -291,10 +301,12 @@ __device__ __noinline__ void exact_slice(Smem& sm, const Part<DT>& p, int top_k)
 // the sort is by key.
 //
 // Memory bounds it for many rows: 2048 x 151936 bf16 with 20 alternatives in
-// 121 us = 5.1 TB/s, 78% of the copy rate (without alternatives 108.6 us, 87%;
+// 120 us = 5.2 TB/s, 79% of the copy rate (without alternatives 107 us, 89%;
 // 223 us when the bound came from the row's beginning and candidates left the
 // loop one by one). The loop runs at the copy rate; what follows it, 20% of a
-// CTA's time, is covered by the SM's other CTAs only in part.
+// CTA's time, is covered by the SM's other CTAs only in part. Instructions more
+// than exponentials count: a quarter of the powers as polynomials of degree 5,
+// off the special-function units, took 132 us.
 template <int DT, int kUnroll>
 __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k) {
   using V = Vec<DT>;
@@ -326,21 +338,23 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
   float top = 0.f;  // the thread's largest value, in vector `at` (the first that holds it)
   int at = -1, entry = 0, in_entry = 0;
   auto take_batch = [&](const uint4 (&r)[kUnroll], int j0, int left) {  // left: vectors from the warp's first on
-    float m[kUnroll];
+    typename V::Max m[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) m[u] = V::vmax(r[u]);
-    float mb = m[0];
+    for (int u = 0; u < kUnroll; ++u) m[u] = V::maxima(r[u]);
+    typename V::Max whole = m[0];
 #pragma unroll
-    for (int u = 1; u < kUnroll; ++u) mb = fmaxf(mb, m[u]);
+    for (int u = 1; u < kUnroll; ++u) whole = V::larger(whole, m[u]);
+    whole = V::across(whole);
+    const float mb = V::value(whole);
     if (top_k > 0) {
       if (at < 0 || mb > top) {
         top = mb;
         int first = kUnroll - 1;
 #pragma unroll
-        for (int u = kUnroll - 2; u >= 0; --u) first = m[u] == mb ? u : first;
+        for (int u = kUnroll - 2; u >= 0; --u) first = V::holds(m[u], whole) ? u : first;
         at = j0 + first * kThreads;
       }
-      __nv_bfloat16 up = __float2bfloat16_ru(mb);
+      __nv_bfloat16 up = V::round_up(whole);
       if (in_entry > 0) up = __hmax(up, sm.batch_max[entry][tid]);
       sm.batch_max[entry][tid] = up;
       if (++in_entry == per) {
@@ -445,7 +459,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
   };
   auto look = [&](int j) {
     const uint4 w = v[j];
-    if (V::vmax(w) < thr) return;
+    if (V::value(V::across(V::maxima(w))) < thr) return;
 #pragma unroll
     for (int i = 0; i < E; ++i) push(top_key(V::raw(w, i), i0 + static_cast<uint32_t>(j) * E + i));
   };
