@@ -180,15 +180,17 @@ class PagedQwen3:
 
         logits = self._logits(self._layers(h, plan, attend))
         picks = lib.token_logprobs(logits, top_k=max(1, self.top_k))
-        # back to the places; padding rows write a place past the last one
-        to = torch.where(plan.token_seq >= 0, place, self.requests)
+        # back to the places; rows without a slot (padding, and places that got no page: those keep the token that is
+        # still to be appended) write a place past the last one
+        to = torch.where(plan.slots >= 0, place, self.requests)
         self.tokens.copy_(torch.cat([self.tokens, self.tokens[:1]]).scatter(0, to, picks.top_ids[:, 0])[:self.requests])
         self.last_places = plan.token_seq
         return logits, picks
 
     def refused(self) -> int:
         """Places of the last decode step that got no slot for their token (no page left, or max_len reached): their row
-        of that step means nothing. Reads the device; the step itself does not."""
+        of that step means nothing, and their length and pending token stay, so that a later step with pages goes on
+        from there. Reads the device; the step itself does not."""
         return int(self.plan_buffers.counts[3])
 
     def release(self, place: int) -> None:

@@ -115,3 +115,27 @@ def test_out_of_pages(model):
     assert server.cache.lens.tolist() == [48, 0]
     with pytest.raises(ValueError, match="no tokens"):
         server.prefill({1: []})
+
+
+def test_a_refused_place_keeps_its_token(cuda):
+    """A place without a page for its pending token keeps that token, and goes on from it once pages come back."""
+    model = qwen3.build(CFG, seed=5, device="cuda")
+    model.norm.weight.data.neg_()  # or random tied weights pick the token that was fed, again and again
+    server = qwen3_paged.PagedQwen3(model, requests=2, max_len=64, pages=4)
+    prompts = {0: prompt(32, 1), 1: prompt(31, 2)}  # all four pages; place 1 has one slot left
+    alone = Alone(model)
+    server.prefill(prompts)
+    alone.feed(prompts[0])
+    first = server.tokens.tolist()
+    server.decode()
+    assert server.refused() == 1 and server.cache.lens.tolist() == [32, 32]
+    second = server.tokens.tolist()
+    assert second[0] == first[0]
+    server.decode()
+    assert server.refused() == 2 and server.tokens.tolist() == second
+    server.release(1)
+    for length in (33, 34):
+        fed = server.tokens.tolist()[0]
+        logits, picks = server.decode()
+        assert server.refused() == 0 and int(server.cache.lens[0]) == length
+        assert near(logits[0], alone.feed([fed])) and int(server.tokens[0]) == int(picks.top_ids[0, 0])
