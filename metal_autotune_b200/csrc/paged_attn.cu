@@ -42,6 +42,11 @@ constexpr int kLeastRun = 6;
 // Warps work by themselves where a request has fewer places than this on average (of 16 keys), and runs are at least so
 // long: 256 requests of 1..512 keys 28.5 us, 34.2 by CTAs; 32 of 1024 33.6, 29.6 by CTAs.
 constexpr int kSoloMean = 24, kSoloRun = 4;
+// The largest probability as a power of 2 where they are rounded to f16, whose normal numbers end at 2^-14: with 1 as the
+// largest, a key 10 nats below it lost bits and one 18 below vanished from the output but not from the sum. So they are
+// whole down to 2^-29 of the largest (20 nats) and 2^-40 of it off at most. Sum, output and a request's parts are in
+// these units, which cancel at the end. (bf16 has fp32's exponents.)
+constexpr float kTopF16 = 15.f;
 constexpr int kMaxCtas = 296;  // bounds the workspace; 2 CTAs on each of 148 SMs
 // arrival counters, one per warp of the grid, in the workspace's control words (the quantised matmul's: both leave
 // them zero, and the workspace is used by one kernel at a time)
@@ -329,7 +334,9 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, int64_t c0, int
 // query rows of a kv head as their 8 columns: S^T = K Q^T, then O^T += V^T P^T,
 // so up to 8 query heads of a kv head fill them without padding, and an
 // accumulator takes D/2 registers. The probabilities are rounded to 16 bits for
-// the product with V; maximum, sum and output stay in fp32.
+// the product with V, since a tensor instruction takes both operands in one
+// type and V has 16 bits: an error of the size of the output's own rounding.
+// Maximum, sum and output stay in fp32.
 //
 // Memory bounds it where contexts are long: 4 flops a byte at 4 query heads to
 // a kv head. Heads of 128, 32/8, bf16, pages of 16: 64 requests of 64..8192
@@ -639,10 +646,11 @@ __global__ void __launch_bounds__(kCtaThreads, kPerSm)
             }
           }
           const float r0 = mx[j][0] == -INFINITY ? 0.f : mx[j][0], r1 = mx[j][1] == -INFINITY ? 0.f : mx[j][1];
+          auto power = [](float z) { return exp2_approx(DT == MT_F16 ? z + kTopF16 : z); };
 #pragma unroll
           for (int kb = 0; kb < NK; ++kb) {
-            const float e0 = exp2_approx(x[kb][0] - r0), e1 = exp2_approx(x[kb][1] - r1);
-            const float e2 = exp2_approx(x[kb][2] - r0), e3 = exp2_approx(x[kb][3] - r1);
+            const float e0 = power(x[kb][0] - r0), e1 = power(x[kb][1] - r1);
+            const float e2 = power(x[kb][2] - r0), e3 = power(x[kb][3] - r1);
             sum[j][0] += e0 + e2;
             sum[j][1] += e1 + e3;
             // the probabilities in 16 bits, as the product with V takes them

@@ -398,6 +398,34 @@ def test_attend_infinities(cuda):
     assert torch.equal(o[2], clean[2])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("below", [12, 15, 17, 20])
+def test_attend_strong_keys_without_a_value(cuda, D, below, dtype):
+    """A few keys draw the attention and hold zeros; the output is what the thousands of keys `below` nats under them
+    (within a quarter) carry, each with a probability far under the type's lowest normal number."""
+    g, dt = gen(below + D), DT[dtype]
+    lens, Hq, Hkv, page = [3900 + 13 * i for i in range(20)], 16, 4, 16
+    q, kc, vc, table, ln = attend_case(lens, Hq, Hkv, D, page, dtype, seed=below)
+    q.zero_()
+    q[..., 0] = 8.0
+    kc[..., 0] = torch.where(torch.isnan(kc[..., 0]), NAN, 0.02 * torch.randn(kc.shape[:-1], generator=g, device="cuda").clamp(-1.5, 1.5)).to(dt)
+    vc.abs_()
+    strong = torch.arange(0, 128, 16, device="cuda")  # one at least for each warp
+    for b in range(len(lens)):
+        at = (table[b, strong // page].long(), slice(None), strong % page)
+        kc[(*at, 0)] = below / 8
+        vc[at] = 0.0
+    o = lib.paged_sdpa_decode(q, kc, vc, table, ln, scale=1.0)
+    ref, mag = attend_ref(q, kc, vc, table, ln, 1.0)
+    # the output's rounding (2^-25 where f16 is subnormal), one of each probability (f16 holds the largest as 2^15, so
+    # 2^-40 of it where they are subnormal, |v| < 8), and fp32 arithmetic on scores of up to 30 in the exponent of 2
+    tol = 1.05 * U[dtype] * (ref.abs() + mag) + 1e-5 * mag
+    if dtype == "f16":
+        tol += 2.0 ** -25 + max(lens) * 8 * 2.0 ** -40
+    assert bool(((o.double() - ref).abs() <= tol).all()), ((o.double() - ref).abs() / tol).max()
+
+
 def test_attend_missing_pages(cuda):
     """Keys on a page id outside the cache are hidden and reported; a length past the table is cut."""
     q, kc, vc, table, ln = attend_case([100, 64], 4, 2, 64, 16, "f16", seed=4)
