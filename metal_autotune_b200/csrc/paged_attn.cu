@@ -270,11 +270,15 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, int64_t c0, int
       float4 v[ROWS][BATCH];
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
-        const int64_t at = min(c + k, c1);
+        const int64_t at = c + k;
         const float* q = p.part + (at * 2 + (at == c0)) * kPart;
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
           const int r = min(r0 + j * apart, rows - 1);
+          m[j][k] = -INFINITY;
+          l[j][k] = 0.f;
+          v[j][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (at > c1) continue;
           m[j][k] = __ldcg(q + r);
           l[j][k] = __ldcg(q + R + r);
           v[j][k] = __ldcg(reinterpret_cast<const float4*>(q + 2 * R + r * D + d));
@@ -284,18 +288,15 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, int64_t c0, int
       for (int j = 0; j < ROWS; ++j) {
         float nm = M[j];
 #pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-          if (c + k > c1) m[j][k] = -INFINITY;
-          nm = fmaxf(nm, m[j][k]);
-        }
-        const float f0 = M[j] == -INFINITY ? 0.f : exp2_approx(M[j] - nm);
+        for (int k = 0; k < BATCH; ++k) nm = fmaxf(nm, m[j][k]);
+        // parts whose maximum is -inf count 0 times what they hold, not nothing: NaN scores leave no maximum but a NaN sum
+        const float ref = nm == -INFINITY ? 0.f : nm, f0 = exp2_approx(M[j] - ref);
         L[j] *= f0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[j][e] *= f0;
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
-          if (m[j][k] == -INFINITY) continue;
-          const float f = exp2_approx(m[j][k] - nm);
+          const float f = exp2_approx(m[j][k] - ref);
           L[j] = fmaf(f, l[j][k], L[j]);
           x[j][0] = fmaf(f, v[j][k].x, x[j][0]);
           x[j][1] = fmaf(f, v[j][k].y, x[j][1]);

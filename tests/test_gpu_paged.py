@@ -426,6 +426,29 @@ def test_attend_strong_keys_without_a_value(cuda, D, below, dtype):
     assert bool(((o.double() - ref).abs() <= tol).all()), ((o.double() - ref).abs() / tol).max()
 
 
+@pytest.mark.parametrize("lens,Hq,Hkv,D,page", [([33333], 32, 8, 128, 16), ([9000, 40], 12, 1, 64, 24),
+                                                ([1 + (2 * i) % 511 for i in range(256)], 32, 8, 128, 16)])
+def test_attend_nan_in_split_requests(cuda, lens, Hq, Hkv, D, page):
+    """A query row or keys of NaN give NaN however many workers (CTAs or warps) share the request, and only in their rows."""
+    q, kc, vc, table, ln = attend_case(lens, Hq, Hkv, D, page, "bf16", seed=17)
+    clean = lib.paged_sdpa_decode(q, kc, vc, table, ln, scale=0.1)
+    bad = q.clone()
+    bad[:, 3, 7] = NAN
+    o = lib.paged_sdpa_decode(bad, kc, vc, table, ln, scale=0.1)
+    others = torch.arange(Hq, device="cuda") != 3
+    assert bool(torch.isnan(o[:, 3]).all()) and torch.equal(o[:, others], clean[:, others])
+    # the first n keys of the last kv head: some n ends where the first worker's run does
+    G, was = Hq // Hkv, kc.clone()
+    for n in [*range(64, min(max(lens), 2600), 64), max(lens)]:
+        for b in range(len(lens)):
+            key = torch.arange(min(n, lens[b]), device="cuda")
+            kc[table[b].long()[key // page], Hkv - 1, key % page, 1] = NAN
+        o = lib.paged_sdpa_decode(q, kc, vc, table, ln, scale=0.1)
+        assert bool(torch.isnan(o[:, -G:]).all()), n
+        assert torch.equal(o[:, :-G], clean[:, :-G])
+        kc.copy_(was)
+
+
 def test_attend_missing_pages(cuda):
     """Keys on a page id outside the cache are hidden and reported; a length past the table is cut."""
     q, kc, vc, table, ln = attend_case([100, 64], 4, 2, 64, 16, "f16", seed=4)
