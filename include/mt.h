@@ -551,8 +551,11 @@ int mt_causal_conv1d(const void* x, const void* weight, const void* bias,
  * when its pages end past the n_free pages of the list; the requests after
  * one that ran out of pages get none either, so pages are dealt in order.
  * The same inputs give the same plan again: no input but the table is
- * written, and only entries past the cached tokens. Output lengths, the head
- * and the counts are the inputs of the next step. Sums saturate at 2^31 - 1.
+ * written, and only entries past the cached tokens. Output lengths and the
+ * head (counts[4]) are the next step's ctx_lens and free_head, by a copy or
+ * with two sets of buffers in turn: an output that overlaps an input, the
+ * table's rows or another output is refused (MT_ERR_INVALID_ARGUMENT), since
+ * inputs are read while outputs are written. Sums saturate at 2^31 - 1.
  */
 int mt_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int64_t B,
                   int32_t* block_table, int64_t table_stride, int64_t max_pages,

@@ -619,6 +619,29 @@ __global__ void __launch_bounds__(kAppendThreads) append_any_kernel(const Append
   }
 }
 
+// ------------------------------------------------------- arguments in memory
+struct Span {
+  const char* name;
+  const void* p;
+  int64_t bytes;
+  bool meets(const Span& o) const {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(o.p);
+    return bytes > 0 && o.bytes > 0 && a < b + o.bytes && b < a + bytes;
+  }
+};
+struct TableSpan {  // rows with room between them, which is not theirs
+  const void* p;
+  int64_t rows, stride, bytes;
+  bool meets(const Span& o) const {
+    if (rows == 0 || bytes == 0 || o.bytes == 0) return false;
+    const int64_t at = static_cast<int64_t>(reinterpret_cast<uintptr_t>(o.p) - reinterpret_cast<uintptr_t>(p));
+    const int64_t end = at + o.bytes;
+    if (at < 0) return end > 0;
+    const int64_t row = at / stride;
+    return row < rows && (at - row * stride < bytes || (row + 1 < rows && end > (row + 1) * stride));
+  }
+};
+
 }  // namespace
 }  // namespace mt
 
@@ -644,6 +667,27 @@ int mt_paged_plan(const int32_t* ctx_lens, const int32_t* new_lens, int64_t B, i
                    (B == 0 || max_pages == 0 || block_table) && (n_free == 0 || free_pages) &&
                    (token_cap == 0 || (positions && token_seq && slots)),
                "mt_paged_plan: null pointer");
+  // CTAs read the inputs while others write: no output may lie over an input, the table or another output
+  {
+    const Span in[] = {{"ctx_lens", ctx_lens, 4 * B}, {"new_lens", new_lens, 4 * B}, {"free_pages", free_pages, 4 * n_free},
+                       {"free_head", free_head, free_head ? 4 : 0}};
+    const Span out[] = {{"seq_lens", seq_lens, 4 * B},          {"query_start", query_start, 4 * (B + 1)},
+                        {"positions", positions, 4 * token_cap}, {"token_seq", token_seq, 4 * token_cap},
+                        {"slots", slots, 8 * token_cap},         {"counts", counts, 20}};
+    const TableSpan table = {block_table, B, 4 * table_stride, 4 * max_pages};
+    const char *one = nullptr, *other = nullptr;
+    for (const Span& i : in)
+      if (table.meets(i)) one = "block_table", other = i.name;
+    for (int k = 0; k < 6; ++k) {
+      if (table.meets(out[k])) one = out[k].name, other = "block_table";
+      for (const Span& i : in)
+        if (out[k].meets(i)) one = out[k].name, other = i.name;
+      for (int l = 0; l < k; ++l)
+        if (out[k].meets(out[l])) one = out[k].name, other = out[l].name;
+    }
+    MT_CHECK_ARG(one == nullptr, "mt_paged_plan: %s overlaps %s in memory (a step's outputs are the next one's inputs by a copy or a second set of buffers)",
+                 one, other);
+  }
   int sms = 148;
   if (int rc = device_sm_count(&sms)) return rc;
   const PlanArgs a = {ctx_lens, new_lens, B, block_table, table_stride, max_pages, free_pages, free_head, n_free,

@@ -604,7 +604,9 @@ def paged_plan(ctx_lens, new_lens, block_table, free_pages, *, page_size, token_
     place with the new pages; free_pages int32 [n], taken from *free_head (int32 [1], default 0) on.
     Returns a PagedPlan (`out`, from PagedPlan.empty(B, token_cap), or a new one): seq_lens [B],
     query_start [B+1], positions / token_seq int32 and slots int64 [token_cap] (slot -1: padding or a
-    refused request), counts [5] = tokens, pages wanted, pages taken, requests refused, next free_head."""
+    refused request), counts [5] = tokens, pages wanted, pages taken, requests refused, next free_head.
+    seq_lens and counts[4:] are the next step's ctx_lens and free_head: pass another `out` there (two in
+    turn), or copies; an output that shares memory with an input is refused."""
     r = _done((_native or native()).paged_plan(ctx_lens, new_lens, block_table, free_pages, page_size, token_cap, free_head,
                                                out), "mt_paged_plan")
     return r if out is not None else PagedPlan._make(r)

@@ -133,6 +133,31 @@ def test_plan_no_requests(cuda):
     assert p.slots.tolist() == [-1, -1, -1] and p.query_start.tolist() == [0] and p.counts.tolist() == [0] * 5
 
 
+def test_plan_step_after_step(cuda):
+    """A step's lengths and head as the next one's inputs, with two sets of outputs in turn; head and lengths in the
+    room beside the table's rows; one set for both is refused."""
+    r = np.random.default_rng(4)
+    B, page, width, cap, n_free = 700, 4, 40, 2600, 20000
+    state = torch.full((B, width + 4), -9, dtype=torch.int32, device="cuda")
+    table = state[:, :width]
+    head = state[B - 1, width + 1:width + 2]
+    head.zero_()
+    free = i32(r.permutation(30000)[:n_free])
+    lens, ref_table, ref_lens, ref_head = i32([0] * B), np.full((B, width), -9), [0] * B, 0
+    sets = [lib.PagedPlan.empty(B, cap) for _ in range(2)]
+    for step in range(6):
+        new = r.integers(0, 6, B)
+        p = lib.paged_plan(lens, i32(new), table, free, page_size=page, token_cap=cap, free_head=head, out=sets[step % 2])
+        ref = plan_ref(ref_lens, list(new), ref_table, free.cpu().numpy(), ref_head, page, cap)
+        for name, got, want in zip(("table",) + lib.PagedPlan._fields, (table, *p), ref):
+            assert np.array_equal(got.cpu().numpy(), np.asarray(want).reshape(got.shape)), (step, name)
+        lens, head = p.seq_lens, p.counts[4:]
+        ref_table, ref_lens, ref_head = ref[0], ref[1], ref[6][4]
+    for kw in (dict(ctx=p.seq_lens, head=None), dict(ctx=sets[0].seq_lens, head=p.counts[4:])):
+        with pytest.raises(lib.MTError, match="overlaps"):
+            lib.paged_plan(kw["ctx"], i32(new), table, free, page_size=page, token_cap=cap, free_head=kw["head"], out=p)
+
+
 # ------------------------------------------------------------------ append
 def cache_pair(pages, Hkv, page, D, dt, layout, fill=0.0):
     shape = (pages, Hkv, page, D) if layout == "hnd" else (pages, page, Hkv, D)

@@ -40,6 +40,40 @@ def test_plan_refuses(mt):
     refused(mt, plan(free=None), -1, b"null pointer")
 
 
+def test_plan_refuses_overlaps(mt):
+    """An output over an input, the table's rows or another output, by address alone."""
+    B, cap, n_free, stride, width = 6, 700, 50, 8, 5
+    at = {}
+    where = 1 << 20
+    for name, size in dict(ctx=4 * B, new=4 * B, table=4 * stride * B, free=4 * n_free, head=4, lens=4 * B, start=4 * (B + 1), pos=4 * cap,
+                           seq=4 * cap, slots=8 * cap, counts=20).items():
+        at[name] = (where, size)
+        where += size + 64 - size % 64
+
+    def plan(**moved):
+        a = {name: C.c_void_p(moved.get(name, p)) for name, (p, _) in at.items()}
+        return mt.mt_paged_plan(a["ctx"], a["new"], B, a["table"], stride, width, a["free"], n_free, a["head"], 16, cap, a["lens"], a["start"],
+                                a["pos"], a["seq"], a["slots"], a["counts"], None)
+
+    outs, ins = ("lens", "start", "pos", "seq", "slots", "counts"), ("ctx", "new", "free", "head")
+    for out in outs:
+        size = at[out][1]
+        for other in (*ins, *(o for o in outs if o != out)):
+            first, n = at[other]
+            refused(mt, plan(**{out: first}), -1, b"overlaps")
+            refused(mt, plan(**{out: first + n - 4}), -1, b"overlaps")
+            refused(mt, plan(**{out: first + 4 - size}), -1, b"overlaps")
+    refused(mt, plan(counts=at["counts"][0], head=at["counts"][0] + 16), -1, b"counts overlaps free_head")
+    refused(mt, plan(ctx=at["lens"][0]), -1, b"seq_lens overlaps ctx_lens")
+    table = at["table"][0]
+    for name in (*ins, "lens", "counts"):
+        n = at[name][1]
+        for row in (0, 3, 5):  # on a row's first entry, its last one, and from before a row into it
+            refused(mt, plan(**{name: table + 4 * stride * row}), -1, b"overlaps")
+            refused(mt, plan(**{name: table + 4 * (stride * row + width - 1)}), -1, b"overlaps")
+            refused(mt, plan(**{name: table + 4 * stride * row + 4 - n}), -1, b"overlaps")
+
+
 def test_append_refuses(mt):
     base = dict(q=P, st=4096, dims=128, page=16, T=2, Hq=32, Hkv=8, D=128, dt=BF, cache=P, inv=P)
 
