@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const PlanArgs a) {
   const int avail = n_free - head;
   const int64_t room = a.max_pages * ps < kPlanMax ? a.max_pages * ps : kPlanMax;
   if (tid < 3) red[tid] = 0;
+  if (a.B == 0) __syncthreads();  // no scan below whose barriers would order it before the sums
   const bool vec = ((reinterpret_cast<uintptr_t>(a.ctx) | reinterpret_cast<uintptr_t>(a.fresh)) & 15) == 0;
   auto pages_of = [&](int len) { return len > 0 ? a.page.div(len - 1) + 1 : 0; };
   int tok_base = 0, page_base = 0, refused = 0, taken = 0;
