@@ -634,6 +634,7 @@ int mt_paged_sdpa_decode(
  * bf16, f16 or f32 in, fp32 out; nothing is rounded to the logits' type
  * (mt_logits_pick does, as mlx-lm). -inf logits have probability 0; a row
  * that holds NaN or +inf, or only -inf, has no distribution and gives NaN.
+ * No log-probability is above 0 and no entropy below, whatever rounding does.
  * 0 <= top_k <= 32.
  */
 int mt_token_logprobs(const void* logits, int64_t row_stride,

@@ -28,7 +28,9 @@ constexpr int kGroups = 64;    // groups of threads whose maxima bound the k-th 
 constexpr int kEntries = 32;   // maxima of its batches that a thread keeps
 constexpr int kCap = 2048;     // candidates kept before the exact form takes over
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr double kLn2 = 0.69314718055994530942;
+// what a unit of the sums' exponents is worth: by the constant that they were scaled with, not by ln 2, or the largest
+// logit would come back 1.3e-8 of itself off (2.7e-4 at 20000)
+constexpr double kUnit = 1.0 / static_cast<double>(kLog2e);
 
 // Larger keys first: the value's order, then the lower index. NaN sorts above
 // every number, -0 equals +0. No element's key is 0.
@@ -165,7 +167,7 @@ __device__ __forceinline__ uint64_t take(uint64_t list, uint64_t rising, int lan
 }
 
 struct Slice {  // what a CTA found in its part of a row
-  double m;    // as m ln 2 of a whole m, or the largest logit itself: exact where the sums' rounding would show
+  double m;    // a whole number of units, or the largest logit itself: neither is rounded to fp32
   float s, t;  // sum e^(x-m), sum e^(x-m) (x-m); s = 0 where every logit is -inf
   uint64_t list[kMaxTop];
 };
@@ -437,9 +439,9 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
     t = warp_sum(f * fmaf(d, s, t));
     s = warp_sum(f * s);
     if (lane == 0) {
-      sm.out.m = static_cast<double>(mb) * kLn2;
+      sm.out.m = static_cast<double>(mb) * kUnit;
       sm.out.s = s;
-      sm.out.t = t * static_cast<float>(kLn2);
+      sm.out.t = t * static_cast<float>(kUnit);
       // the largest value alone adds over 1/2, unless it lies below kFloor or the row holds NaN or +inf
       sm.exact = !(s >= 0.25f && s < INFINITY && t == t);
     }
@@ -560,18 +562,24 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
   if (tid >= 32) return;
   const float ls = s > 0.f ? logf(s) : NAN;  // no distribution: NaN throughout
   const double lse = m + ls;
+  // of a token that carries the row, rounding (the powers': 2^-22) can put the logarithm, and the entropy, past 0
+  auto log_prob = [&](float x) {
+    const float lp = static_cast<float>(x - lse);
+    return lp > 0.f ? 0.f : lp;
+  };
   if (lane == 0) {
     if (a.lse) a.lse[row] = static_cast<float>(lse);
-    if (a.entropy) a.entropy[row] = ls - t / s;
+    const float entropy = ls - t / s;
+    if (a.entropy) a.entropy[row] = entropy < 0.f ? 0.f : entropy;
     if (a.tokens) {
       const int tok = a.tokens[row];
       if (tok >= a.V) report_status(0x801);
-      a.logprob[row] = tok >= 0 && tok < a.V ? static_cast<float>(Elem<DT>::to_f(p.x[tok]) - lse) : 0.f;
+      a.logprob[row] = tok >= 0 && tok < a.V ? log_prob(Elem<DT>::to_f(p.x[tok])) : 0.f;
     }
   }
   if (lane < a.top_k) {
     a.top_ids[row * a.top_k + lane] = key_index(list);
-    a.top_lp[row * a.top_k + lane] = static_cast<float>(key_value(list) - lse);
+    a.top_lp[row * a.top_k + lane] = log_prob(key_value(list));
   }
 }
 

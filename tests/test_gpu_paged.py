@@ -582,6 +582,30 @@ def test_logprobs_ties_masks_and_extremes(cuda, dtype):
         check_logprobs(x, [0, 7, 3, 12345, 0, 0, 39998, 1, 50, 2, 30000, 9], k)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("R", [1, 700])
+def test_logprobs_of_a_certain_token(cuda, dtype, R):
+    """One value carries the row: its log-probability is 0 but for the rest's share, however large the logit, and no
+    log-probability is positive."""
+    V, dt = 20000, DT[dtype]
+    rows = [(30.0, 0.0), (600.0, 0.0), (20000.0, 1.0), (60000.0, -100.0), (-20000.0, -INF), (-100.0, -140.0), (33.3, 0.0), (25.7, -3.0)]
+    for r0 in range(0, len(rows), 1 if R == 1 else len(rows)):
+        pairs = [rows[r0]] if R == 1 else [rows[i % len(rows)] for i in range(R)]
+        x = torch.tensor([low for _, low in pairs], device="cuda")[:, None].repeat(1, V)
+        ids = [(7919 * i + 11) % V for i in range(R)]
+        x[torch.arange(R), ids] = torch.tensor([high for high, _ in pairs], device="cuda")
+        x = x.to(dt)
+        p = lib.token_logprobs(x, i32(ids), top_k=2)
+        with np.errstate(all="ignore"):
+            lp, H, _, _, top = logprob_ref(x, ids, 2)
+        # the power's error, 2^-22, and a few roundings of numbers up to 1; none of the logit's size
+        for got, want in ((p.logprob, lp), (p.top_logprobs[:, 0], top[:, 0])):
+            assert np.all(np.abs(got.double().cpu().numpy() - want) <= 2.0 ** -21)
+            assert bool((got <= 0).all())
+        assert bool((p.top_logprobs <= 0).all()) and bool((p.entropy >= 0).all())
+        assert np.all(np.abs(p.entropy.double().cpu().numpy() - H) <= 2.0 ** -20)
+
+
 def test_logprobs_no_distribution(cuda):
     V = 5000
     x = torch.randn(5, V, generator=gen(2), device="cuda")
