@@ -105,21 +105,27 @@ def build_graph_library(force: bool = False) -> Path:
 
 BIND_SRC = CSRC / "bind.cpp"
 BIND_LIB = LIBDIR / "mt_bind.so"
+BIND_STAMP = OBJDIR / "mt_bind.stamp"  # what the module was built for
 
 
 def build_bind_library(force: bool = False) -> Path:
     """Compile csrc/bind.cpp (a Python extension module over torch's C++
-    tensors that calls libmt.so beside it) into lib/mt_bind.so; returns its path."""
-    build_library()
-    deps = [BIND_SRC, INCLUDE / "mt.h", Path(__file__)]
-    if not force and not _stale(BIND_LIB, deps):
-        return BIND_LIB
+    tensors that calls libmt.so beside it) into lib/mt_bind.so, again where
+    torch or Python is not the one it was built for; returns its path."""
     import sysconfig
 
     import torch
+    build_library()
+    # a module built against one torch (or Python) must not be loaded into another
+    stamp = f"torch {torch.__version__} {torch.version.git_version}, python {sys.version}\n"
+    deps = [BIND_SRC, INCLUDE / "mt.h", Path(__file__)]
+    built_for = BIND_STAMP.read_text() if BIND_STAMP.exists() else None
+    if not force and not _stale(BIND_LIB, deps) and built_for == stamp:
+        return BIND_LIB
     cxx = shutil.which("g++") or shutil.which("c++")
     if cxx is None:
         raise RuntimeError("no C++ compiler; mt_bind.so cannot be built")
+    BIND_STAMP.unlink(missing_ok=True)
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parents[1]
     inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
@@ -133,6 +139,8 @@ def build_bind_library(force: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {BIND_SRC.name}:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, BIND_LIB)
+    BIND_STAMP.parent.mkdir(exist_ok=True)
+    BIND_STAMP.write_text(stamp)
     return BIND_LIB
 
 

@@ -178,6 +178,26 @@ def test_wrappers_check_their_tensors(monkeypatch):
         lib.token_logprobs(z(4, 10), i(4))
 
 
+def test_binding_is_built_for_this_torch(monkeypatch, tmp_path):
+    """A module that is newer than its source but was built for another torch is compiled again."""
+    build.build_bind_library()
+    built_for = build.BIND_STAMP.read_text()
+    assert torch.__version__ in built_for
+    compiled = []
+
+    class Failed:
+        returncode, stdout, stderr = 1, "", "not compiled in this test"
+
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, **kw: compiled.append(cmd) or Failed)
+    monkeypatch.setattr(build, "BIND_STAMP", tmp_path / "stamp")
+    build.BIND_STAMP.write_text(built_for)
+    assert build.build_bind_library() == build.BIND_LIB and not compiled
+    build.BIND_STAMP.write_text(built_for.replace(torch.__version__, "0.0"))
+    with pytest.raises(RuntimeError, match="not compiled in this test"):
+        build.build_bind_library()
+    assert len(compiled) == 1 and not build.BIND_STAMP.exists()
+
+
 # ------------------------------------------------------------------ rotary frequencies
 def test_frequencies_without_scaling():
     f, m = lib.rope_frequencies(8, base=10000.0, device="cpu")
