@@ -231,6 +231,11 @@ def test_append(cuda, T, Hq, Hkv, D, dims, trad, norm, dtype, page, layout, max_
     assert lib.device_status() == 0
 
 
+@pytest.mark.parametrize("dims,trad,norm", [(128, False, True), (64, True, False)])
+def test_append_many_f32_rows(cuda, dims, trad, norm):
+    test_append(cuda, 900, 8, 2, 128, dims, trad, norm, "f32", 16, "hnd", 5000)
+
+
 def test_append_matches_dense_rope(cuda):
     """Without norm or scaling: the same rotation as mt_rope at each token's position, up to one rounding step."""
     g, T, H, D = gen(3), 9, 4, 128
