@@ -27,6 +27,7 @@ constexpr int kUnrollMany = 4, kUnrollFew = 8, kCtasPerSmFew = 4;
 constexpr int kGroups = 64;    // groups of threads whose maxima bound the k-th largest value
 constexpr int kEntries = 32;   // maxima of its batches that a thread keeps
 constexpr int kCap = 2048;     // candidates kept before the exact form takes over
+constexpr int kNothingSeen = 2;  // Smem::exact: sums of 0, no NaN: only -inf, or values far below kFloor too
 constexpr float kLog2e = 1.4426950408889634f;
 // what a unit of the sums' exponents is worth: by the constant that they were scaled with, not by ln 2, or the largest
 // logit would come back 1.3e-8 of itself off (2.7e-4 at 20000)
@@ -180,7 +181,7 @@ struct Smem {
   __nv_bfloat16 batch_max[kEntries][kThreads];
   float red[3][kWarps];
   double red_d[2][kWarps];
-  int count, hits, exact;
+  int count, hits, exact;  // exact: the sums of one pass will not do
   Slice out;
 };
 
@@ -219,10 +220,40 @@ struct Part {
   __device__ __forceinline__ const uint4* vec() const { return reinterpret_cast<const uint4*>(x + body); }
 };
 
-// Any input, several passes: every logit -inf or tiny, NaN, +inf, or more
-// candidates than the buffer holds (values that keep rising along the row).
+// A part of nothing but -inf, as a mask that allows one range of ids leaves
+// beside it: no sums, and its first values as the candidates. True if it is one.
+// (By the exact form below, with a barrier for each 256 values, such a part held
+// up its row: a hundredth of 151936 ids in one range took 79 us for one row and
+// 305 for 256, where as many anywhere in the row take 9 and 25.)
+template <int DT>
+__device__ __forceinline__ bool empty_slice(Smem& sm, const Part<DT>& p) {
+  using V = Vec<DT>;
+  const int tid = threadIdx.x;
+  const int64_t a0 = p.body + p.v0 * V::E, n_body = (p.v1 - p.v0) * V::E;
+  bool other = false;  // (a NaN beside -inf does not show in a maximum, but the caller has seen none)
+#pragma unroll 4
+  for (int64_t j = p.v0 + tid; j < p.v1; j += kThreads)
+    other |= V::value(V::across(V::maxima(p.vec()[j]))) != -INFINITY;
+  if (tid < p.head) other |= Elem<DT>::to_f(p.x[tid]) != -INFINITY;
+  if (tid < p.tail) other |= Elem<DT>::to_f(p.x[p.tail0 + tid]) != -INFINITY;
+  if (__syncthreads_or(other)) return false;
+  if (tid < 32) {
+    const int64_t b = tid - p.head, t = b - n_body;
+    const int64_t i = b < 0 ? tid : t < 0 ? a0 + b : t < p.tail ? p.tail0 + t : -1;
+    sm.out.list[tid] = i >= 0 ? top_key(-INFINITY, static_cast<uint32_t>(i)) : 0;
+  }
+  if (tid == 0) {
+    sm.out.m = -INFINITY;
+    sm.out.s = sm.out.t = 0.f;
+  }
+  return true;
+}
+
+// Any input, several passes: every logit tiny, NaN, +inf, or more candidates
+// than the buffer holds (values that keep rising along the row).
 template <int DT>
 __device__ __noinline__ void exact_slice(Smem& sm, const Part<DT>& p, int top_k) {
+  if (sm.exact == kNothingSeen && empty_slice<DT>(sm, p)) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int E = Vec<DT>::E;
   const int64_t a0 = p.body + p.v0 * E, n_body = (p.v1 - p.v0) * E;
@@ -443,7 +474,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
       sm.out.s = s;
       sm.out.t = t * static_cast<float>(kUnit);
       // the largest value alone adds over 1/2, unless it lies below kFloor or the row holds NaN or +inf
-      sm.exact = !(s >= 0.25f && s < INFINITY && t == t);
+      sm.exact = s >= 0.25f && s < INFINITY && t == t ? 0 : s == 0.f && t == 0.f ? kNothingSeen : 1;
     }
   };
   if (top_k == 0) {
@@ -476,6 +507,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
       if (h < kHits) hits[h] = e * span + tid;
     }
   __syncthreads();
+  if (sm.exact) return false;
   if (sm.hits <= kHits) {
     for (int i = tid; i < sm.hits * per * kUnroll; i += kThreads) {
       const int h = i / (per * kUnroll), j = hits[h] + (i - h * per * kUnroll) * kThreads;
@@ -488,7 +520,7 @@ __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k)
   }
   if (extra_i >= 0) push(top_key(extra, static_cast<uint32_t>(extra_i)));
   __syncthreads();
-  if (sm.exact || sm.count > kCap) return false;
+  if (sm.count > kCap) return false;
   // top 32 of the candidates: batches of 32 sorted by the warps, their lists joined in pairs
   const int c = sm.count;
   uint64_t list = 0;
