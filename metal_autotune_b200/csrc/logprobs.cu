@@ -27,7 +27,7 @@ constexpr int kUnrollMany = 4, kUnrollFew = 8, kCtasPerSmFew = 4;
 constexpr int kGroups = 64;    // groups of threads whose maxima bound the k-th largest value
 constexpr int kEntries = 32;   // maxima of its batches that a thread keeps
 constexpr int kCap = 2048;     // candidates kept before the exact form takes over
-constexpr int kNothingSeen = 2;  // Smem::exact: sums of 0, no NaN: only -inf, or values far below kFloor too
+constexpr int kNothingSeen = 2;  // Smem::exact: sums of 0, no NaN: every value is -inf or far below kFloor
 constexpr float kLog2e = 1.4426950408889634f;
 // what a unit of the sums' exponents is worth: by the constant that they were scaled with, not by ln 2, or the largest
 // logit would come back 1.3e-8 of itself off (2.7e-4 at 20000)
@@ -220,31 +220,39 @@ struct Part {
   __device__ __forceinline__ const uint4* vec() const { return reinterpret_cast<const uint4*>(x + body); }
 };
 
-// A part of nothing but -inf, as a mask that allows one range of ids leaves
-// beside it: no sums, and its first values as the candidates. True if it is one.
-// (By the exact form below, with a barrier for each 256 values, such a part held
-// up its row: a hundredth of 151936 ids in one range took 79 us for one row and
-// 305 for 256, where as many anywhere in the row take 9 and 25.)
+// A part of one value throughout, as a mask (-inf, or the type's lowest value)
+// that allows one range of ids leaves beside it: the sums are known, and its
+// first values are the candidates. True if it is one. (By the exact form below,
+// with a barrier for each 256 values, such a part held up its row: a hundredth of
+// 151936 ids in one range took 79 us for one row and 305 for 256, where as many
+// anywhere in the row take 9 and 25.)
 template <int DT>
-__device__ __forceinline__ bool empty_slice(Smem& sm, const Part<DT>& p) {
+__device__ __forceinline__ bool constant_slice(Smem& sm, const Part<DT>& p) {
   using V = Vec<DT>;
   const int tid = threadIdx.x;
   const int64_t a0 = p.body + p.v0 * V::E, n_body = (p.v1 - p.v0) * V::E;
-  bool other = false;  // (a NaN beside -inf does not show in a maximum, but the caller has seen none)
+  const int64_t n = n_body + p.head + p.tail;
+  if (n == 0) return false;
+  const float c = Elem<DT>::to_f(p.x[n_body > 0 ? a0 : p.head > 0 ? 0 : p.tail0]);
+  bool other = false;
 #pragma unroll 4
-  for (int64_t j = p.v0 + tid; j < p.v1; j += kThreads)
-    other |= V::value(V::across(V::maxima(p.vec()[j]))) != -INFINITY;
-  if (tid < p.head) other |= Elem<DT>::to_f(p.x[tid]) != -INFINITY;
-  if (tid < p.tail) other |= Elem<DT>::to_f(p.x[p.tail0 + tid]) != -INFINITY;
+  for (int64_t j = p.v0 + tid; j < p.v1; j += kThreads) {
+    const uint4 w = p.vec()[j];
+#pragma unroll
+    for (int e = 0; e < V::E; ++e) other |= V::raw(w, e) != c;
+  }
+  if (tid < p.head) other |= Elem<DT>::to_f(p.x[tid]) != c;
+  if (tid < p.tail) other |= Elem<DT>::to_f(p.x[p.tail0 + tid]) != c;
   if (__syncthreads_or(other)) return false;
   if (tid < 32) {
     const int64_t b = tid - p.head, t = b - n_body;
     const int64_t i = b < 0 ? tid : t < 0 ? a0 + b : t < p.tail ? p.tail0 + t : -1;
-    sm.out.list[tid] = i >= 0 ? top_key(-INFINITY, static_cast<uint32_t>(i)) : 0;
+    sm.out.list[tid] = i >= 0 ? top_key(c, static_cast<uint32_t>(i)) : 0;
   }
   if (tid == 0) {
-    sm.out.m = -INFINITY;
-    sm.out.s = sm.out.t = 0.f;
+    sm.out.m = c;
+    sm.out.s = c == -INFINITY ? 0.f : static_cast<float>(n);
+    sm.out.t = 0.f;
   }
   return true;
 }
@@ -253,7 +261,7 @@ __device__ __forceinline__ bool empty_slice(Smem& sm, const Part<DT>& p) {
 // than the buffer holds (values that keep rising along the row).
 template <int DT>
 __device__ __noinline__ void exact_slice(Smem& sm, const Part<DT>& p, int top_k) {
-  if (sm.exact == kNothingSeen && empty_slice<DT>(sm, p)) return;
+  if (sm.exact == kNothingSeen && constant_slice<DT>(sm, p)) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int E = Vec<DT>::E;
   const int64_t a0 = p.body + p.v0 * E, n_body = (p.v1 - p.v0) * E;

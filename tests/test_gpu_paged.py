@@ -657,6 +657,36 @@ def test_logprobs_range_costs_what_scattered_ids_cost(cuda, R, k):
     assert one_range < 3 * scattered, (one_range, scattered)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_logprobs_range_among_lowest_values(cuda, dtype):
+    """The same where a mask writes the type's lowest value instead of -inf; parts of one very low value, and a row of it."""
+    R, V, n, dt = 4, 151936, 1519, DT[dtype]
+    low = torch.finfo(dt).min
+
+    def least(x):
+        times = []
+        for _ in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(20):
+                lib.token_logprobs(x, top_k=20)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    took = []
+    for ids in (torch.arange(70000, 70000 + n, device="cuda"), torch.randperm(V, generator=gen(2), device="cuda")[:n]):
+        x = torch.full((R, V), low, dtype=dt, device="cuda")
+        x[:, ids] = torch.randn(R, n, generator=gen(1), device="cuda").to(dt)
+        took.append(least(x))
+        x[1] = low
+        x[2] = -50000.0
+        x[3, :100000] = -40000.0
+        check_logprobs(x, [int(ids[0]), 5, 151935, 7], 20)
+    assert took[0] < 3 * took[1], took
+
+
 def test_logprobs_no_distribution(cuda):
     V = 5000
     x = torch.randn(5, V, generator=gen(2), device="cuda")
