@@ -341,13 +341,14 @@ __device__ __noinline__ void exact_slice(Smem& sm, const Part<DT>& p, int top_k)
 // Which thread stores a candidate where does not matter: keys are unique and
 // the sort is by key.
 //
-// Memory bounds it for many rows: 2048 x 151936 bf16 with 20 alternatives in
-// 120 us = 5.2 TB/s, 79% of the copy rate (without alternatives 107 us, 89%;
-// 223 us when the bound came from the row's beginning and candidates left the
-// loop one by one). The loop runs at the copy rate; what follows it, 20% of a
-// CTA's time, is covered by the SM's other CTAs only in part. Instructions more
-// than exponentials count: a quarter of the powers as polynomials of degree 5,
-// off the special-function units, took 132 us.
+// Many rows: 2048 x 151936 bf16 with 20 alternatives in 120 us = 5.2 TB/s, 79%
+// of the copy rate (223 us when the bound came from the row's beginning and
+// candidates left the loop one by one). Instructions and the ends of rows bound
+// it, not memory: issue slots are 67% busy, DRAM 61%. What follows the loop, 20%
+// of a CTA's time, is covered by the SM's other CTAs only in part: without
+// alternatives 107 us, 89%. A quarter of the powers as polynomials of degree 5,
+// off the special-function units, took 132 us; and call after call under the
+// power limit, at a lower clock, the 120 become 127 to 135.
 template <int DT, int kUnroll>
 __device__ __forceinline__ bool one_pass(Smem& sm, const Part<DT>& p, int top_k) {
   using V = Vec<DT>;

@@ -70,7 +70,7 @@ struct PlanArgs {
 // token on a new page takes the page from the free list directly, so no CTA
 // reads a table entry that another one writes. Latency bounds it: lengths,
 // scans, then a table or free-list entry for each token. 8 requests 3.6 us
-// (6.8 with 64-bit divisions), 4096 requests with 131072 token places 8.9 us
+// (6.8 with 64-bit divisions), 4096 requests with 131072 token places 9.0 us
 // (9.2 with 512 threads of eight requests, 9.8 while those met in shared-memory
 // banks), where the 2.2 MB it moves would take 0.3.
 template <int kThreads, int kItems>
@@ -288,8 +288,8 @@ __device__ __forceinline__ void store8(typename Elem<DT>::T* p, const float (&x)
 }
 
 // Three rows to a group of lanes, two stages, 5 CTAs of 128 threads per SM (91 registers, 24 KB of ring each): 8192
-// tokens of 32/8 heads of 128 with norms in 36.7 us = 5.5 TB/s, 84% of the copy rate. 6 CTAs, or a third stage, 38.6 to
-// 38.9; 4 with three stages 38.3.
+// tokens of 32/8 heads of 128 with norms in 36.7 us = 5.5 TB/s, 84% of the copy rate, in replays of a graph (38.4 to 40.1
+// call after call). 6 CTAs, or a third stage, 38.6 to 38.9; 4 with three stages 38.3.
 constexpr int kAppendRows = 3;
 constexpr int kAppendStages = 2;
 constexpr int kAppendCtas = 5;

@@ -36,8 +36,11 @@ constexpr int kCtaThreads = 2 * kThreads;
 // 64..8192 keys 85.6 us without, 80.3 with 1, 78.4 with 2 or 3; 256 of 1..512 40.8, 29.9, 28.4, 27.7; 37 of 0..1500
 // with 20 heads of 64 17.8 with 2, 15.1 with 3 (and the next rule).
 constexpr int kUnitCost = 3;
-// The least run of a CTA, in places, where requests are that long: one request of 129 keys 6.1 us (a CTA to a head, no
-// parts to join), 7.1 cut at every step; four of 4096 the same either way.
+// The least run of a CTA, in places, where requests are that long. One request of 32/8 heads of 128 at least runs of 1, 3,
+// 6 and 12: 129 keys 7.3, 7.0, 5.7 and 5.8 us (from 6 on a CTA to a head, no parts to join), 512 keys 7.5, 8.4, 9.8, 7.7;
+// 1024 7.8, 8.9, 11.4, 11.4; 4096 10.1, 10.5, 12.2, 17.4; 16384 17.7, 17.8, 17.8, 19.2; four of 4096 keys 16.7 up to 6,
+// 18.5. So 6 serves requests of a step or two, decides those up to some 13000 keys, and costs single ones of 512 to 4096
+// 2 to 3.5 us.
 constexpr int kLeastRun = 6;
 // Warps work by themselves where a request has fewer places than this on average (of 16 keys), and runs are at least so
 // long: 256 requests of 1..512 keys 28.5 us, 34.2 by CTAs; 32 of 1024 33.6, 29.6 by CTAs.
@@ -342,7 +345,7 @@ __device__ __forceinline__ void join_parts(const PagedParams& p, int64_t c0, int
 // Memory bounds it where contexts are long: 4 flops a byte at 4 query heads to
 // a kv head. Heads of 128, 32/8, bf16, pages of 16: 64 requests of 64..8192
 // keys 75 us = 6.0 TB/s, 92% of the copy rate (92.5 us with one warp doing
-// both, by 16-byte copies); one of 131072 87 us, 94%. Few or short requests
+// both, by 16-byte copies); one of 131072 88 us, 93%. Few or short requests
 // wait for a chain of loads (lengths, page, keys: 2.6 us before the first
 // product) and the joins of split requests (1.5 us): one of 129 keys 5.8 us.
 template <int DT, int D, int R, int KEYS, int kStages, bool BOX, int kPerSm>
@@ -882,9 +885,12 @@ int mt_paged_sdpa_decode(const void* q, int64_t q_sb, int64_t q_sh, const void* 
     box = box && extent[i] < (1ll << 32) && (extent[i] == 1 || (bytes[i] > 0 && bytes[i] < (1ll << 40)));
   }
   // Steps of 32 keys for heads of 64, and for heads of 128 where there are few units: then one CTA to an SM, fewer parts
-  // to join and more bytes to a copy of the copy engine. 64 requests of 64..8192 keys (512 units) 77.2 -> 75.6 us, four
-  // of 4096 18.9 -> 16.9, one of 131072 90.6 -> 87.8; but 128 of 64..2048 (1024 units) 55.0 -> 58.4, 256 of 1..512 26.7
-  // -> 29.1, and by 16-byte copies 16 of 64..2048 15.4 -> 16.6.
+  // to join and more bytes to a copy of the copy engine. With 8 units to a request, 16 keys a step against 32: 64..8192
+  // keys 16 requests 25.4 and 24.2 us, 64 77.3 and 74.5, 128 146 and 143; four of 4096 18.9 and 16.9, one of 131072 90.6
+  // and 87.8, 96 of 4096 251 and 247. But 64..2048 keys 16 requests 13.9 and 14.9, 64 31.6 and 34.3, 256 101 and 107; 1..512
+  // keys 64 13.6 and 13.1, 256 26.3 and 28.7; and by 16-byte copies 16 of 64..2048 15.4 and 16.6. It is the lengths and
+  // their spread that decide, which the host does not know; many units stand for short ragged requests here, 3% to 8%
+  // off where they are few and short or many and long.
   const bool wide = D == 64 || (R == 8 && box && B * Hkv * RB <= 512);
   p.box_rows = wide && page_size % 32 == 0 ? 32 : page_size % 16 == 0 ? 16 : 8;
   CUtensorMap kmap = {}, vmap = {};
